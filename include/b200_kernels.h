@@ -26,6 +26,7 @@ extern "C" {
 #define B200_DT_F16 10  /* PJRT_Buffer_Type_F16 */
 #define B200_DT_F32 11  /* PJRT_Buffer_Type_F32 */
 #define B200_DT_BF16 13 /* PJRT_Buffer_Type_BF16 */
+#define B200_DT_S8 2    /* PJRT_Buffer_Type_S8 */
 #define B200_DT_S32 4   /* PJRT_Buffer_Type_S32 */
 #define B200_DT_S64 5   /* PJRT_Buffer_Type_S64 */
 
@@ -48,6 +49,46 @@ B200_API int b200_gemm(const void* A, const void* B, void* C, int64_t batch, int
 B200_API size_t b200_gemm_split_scratch_bytes(int64_t batch, int64_t M, int64_t N, int64_t K, int a_type, int b_type);
 B200_API int b200_gemm_split(const void* A, int a_type, const void* B, int b_type, void* C, int64_t batch, int64_t M,
                              int64_t N, int64_t K, int out_type, void* scratch, size_t scratch_bytes, void* stream);
+
+/* 8-bit linear layer: b200_quantize_i8 and b200_rms_norm_i8 make rows of 8-bit integers with an f32 scale
+ * each (of activations: a scale per token; of a weight matrix [N, K]: a scale per output channel), and
+ * b200_gemm_i8 multiplies two such operands.  Row pitches ld* count elements of their own array; rows
+ * may start at any element, and those whose addresses and pitches are multiples of 16 bytes (q: 8) are
+ * read and written fastest.  Bytes between a row's end and the next row are neither read nor written.
+ * All three only queue work on `stream`, which with every pointer belongs to the current device, and
+ * may be captured.  They return 0, -1 (bad arguments), -2 (no tensor map), -3 (launch failure), or -4
+ * (scratch too small or misaligned).  No counterpart in the reference, whose products are floating. */
+
+/* q[i][j] = round_half_even(127 x[i][j] / max_j |x[i][j]|), the exact quotient's rounding, and scale[i] =
+ * max_j |x[i][j]| / 127, so x is about q * scale.  dtype (of x) in {F32, BF16, F16}.  A row of zeros gives
+ * scale 0 and q 0, a row holding an infinity or a NaN scale NaN and q 0.  rows or cols may be 0. */
+B200_API int b200_quantize_i8(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows,
+                              int64_t cols, int dtype, void* stream);
+
+/* Root-mean-square norm with the residual's addition, rounded to 8 bits: h = x + residual rounded to
+ * dtype (h = x without one), t = f32(h * weight), q = round_half_even(127 t / max_j |t|) as above, scale =
+ * max_j |t| / 127 / sqrt(mean_j h^2 + eps), so the normalised row is about q * scale.  weight [cols] of
+ * weight_dtype; x, residual and h of dtype, each in {F32, BF16, F16}.  residual may be NULL, and then h is
+ * NULL too; with a residual h may be NULL (not written), or x or residual themselves with their pitch.
+ * eps > 0.  A row whose t holds an infinity or a NaN gives scale NaN and q 0.  rows may be 0. */
+B200_API int b200_rms_norm_i8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* h,
+                              int64_t ldh, int8_t* q, int64_t ldq, float* scale, int64_t rows, int64_t cols, int dtype,
+                              int weight_dtype, float eps, void* stream);
+
+/* C[i][j] = act(f32(sum_k A[i][k] B[j][k]) a_scale[i] b_scale[j] + bias[j]): A [M, K] and B [N, K] of 8-bit
+ * integers, K contiguous, the sum exact in 32 bits (K <= 131071), C [M, N] of out_type in {F32, BF16, F16},
+ * act B200_ACT_NONE or B200_ACT_GELU (its tanh form).  a_scale [M], b_scale [N] and bias [N] are f32 and may
+ * each be NULL (1, 1, 0).  out_type S32 gives the sums themselves, without scales, bias or act.  Any of M, N,
+ * K may be 0.  An operand whose address or pitch is no multiple of 16 bytes is first copied to such rows in
+ * `scratch`, 256-byte aligned device memory of b200_gemm_i8_scratch_bytes(...) bytes for these operands (0
+ * when both lie so: scratch may be NULL); calls that overlap on the GPU need a scratch each. */
+#define B200_ACT_NONE 0
+#define B200_ACT_GELU 1
+B200_API size_t b200_gemm_i8_scratch_bytes(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N,
+                                           int64_t K);
+B200_API int b200_gemm_i8(const void* A, int64_t lda, const void* B, int64_t ldb, const float* a_scale,
+                          const float* b_scale, const float* bias, void* C, int64_t ldc, int64_t M, int64_t N, int64_t K,
+                          int out_type, int act, void* scratch, size_t scratch_bytes, void* stream);
 
 /* O = softmax(scale * Q K^T [causal mask]) V, fp32 softmax, for bf16 Q, K, V, O of shape [B, H, S, D]
  * (D contiguous), D = 64, S a multiple of 256.  Fused flash-style kernel on tcgen05; allocates nothing.

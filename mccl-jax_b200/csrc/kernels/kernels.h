@@ -48,6 +48,20 @@ int GemmSplit(const void* A, long long lda, bool a_mn, int a_type, const void* B
               void* C, int64_t batch, int64_t M, int64_t N, int64_t K, int out_type, cudaStream_t st, void* scratch,
               size_t scratch_bytes, int64_t ldc, int* counter = nullptr);
 
+// ---- 8-bit linear layer (quant_rows.cu, gemm_i8.cu) ----------------------------------------------
+// The internal forms of b200_quantize_i8, b200_rms_norm_i8 and b200_gemm_i8 (include/b200_kernels.h).
+// 128 * 128 * kGemmI8MaxK is the largest sum a 32-bit integer holds.
+constexpr int64_t kGemmI8MaxK = 131071;
+int QuantizeI8(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int64_t cols, int dtype,
+               cudaStream_t st);
+int RmsNormI8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* h, int64_t ldh,
+              int8_t* q, int64_t ldq, float* scale, int64_t rows, int64_t cols, int dtype, int weight_dtype, float eps,
+              cudaStream_t st);
+size_t GemmI8ScratchBytes(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K);
+int GemmI8(const void* A, int64_t lda, const void* B, int64_t ldb, const float* a_scale, const float* b_scale, const float* bias,
+           void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, int out_type, int act, void* scratch, size_t scratch_bytes,
+           cudaStream_t st);
+
 // ---- attention (attention_tc.cu, attention_bwd_tc.cu) -------------------------------------------
 bool AttentionShapeOk(int B, int H, int S, int D);
 int AttentionFwd(const void* q, const void* k, const void* v, void* o, int B, int H, int S, int D, int causal, float scale,
