@@ -74,7 +74,8 @@ extern "C" int b200_take_device_error(void) {
   int a = b200k::TakeAttnError();
   int b = b200k::TakeAttnBwdError();
   int t = b200k::TakeSelftestError();
-  return e ? e : a ? a : b ? b : t;
+  int i = b200k::TakeGemmI8Error();
+  return e ? e : a ? a : b ? b : i ? i : t;
 }
 
 extern "C" int b200_selftest_wait_timeout(long long budget_cycles, int* waited_out, void* stream) {

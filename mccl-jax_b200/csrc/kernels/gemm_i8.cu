@@ -1,19 +1,47 @@
 // gemm_i8.cu — products of 8-bit integers with a scale per row of each operand:
 //     C[i][j] = act(f32(sum_k A[i][k] B[j][k]) * a_scale[i] * b_scale[j] + bias[j])
-// with the sum exact in 32-bit integers, and the raw sums themselves (s32 C).
+// with the sum exact in 32-bit integers, and the raw sums themselves (s32 C).  A [M, K] holds tokens, B [N, K]
+// output channels.
+//
+// Two kernels on the integer form of tcgen05 (128-byte rows of K per stage, in the 128-byte swizzle TMA writes):
+//   gemm_i8_pair_kernel   256 tokens x 256 channels on a pair of CTAs, persistent, two accumulators in tensor
+//                         memory so that one tile's stores overlap the next tile's products: many tokens.
+//   gemm_i8_tile_kernel   128 channels x 32, 64 or 128 tokens on one CTA.  Channels are the rows of the tensor
+//                         core's tile, so few tokens leave none of it idle that would have to be fed, and the
+//                         K range may be cut over a cluster of up to 8 CTAs, which add their integer sums
+//                         through distributed shared memory: the sums are exact, so the cut changes no result,
+//                         and neither scratch nor atomics are needed.
+// An operand that TMA cannot read (address or pitch no multiple of 16 bytes) is first copied to rows it can.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
+#include <cstdio>
+#include <cstdlib>
 
 #include "kernels.h"
+#include "tc_common.cuh"
 #include "../../../include/b200_kernels.h"
 
 namespace b200k {
+
+static __device__ int g_tc_error_gemm_i8;
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn GetEncodeTiled();
+
 namespace {
 
 enum : int { kOutF32 = 0, kOutBF16 = 1, kOutF16 = 2, kOutS32 = 3 };
+template <int OUT>
+constexpr int kOutBytes = OUT == kOutF32 || OUT == kOutS32 ? 4 : 2;
+
+constexpr int BK = 128;                          // K bytes per stage: one 128-byte swizzle row
+constexpr int kThreads = 192;                    // TMA warp, MMA warp, four epilogue warps
 
 // What follows the integer sum.  Null scales are 1, a null bias 0.
 struct Epilogue {
@@ -36,52 +64,587 @@ __device__ __forceinline__ float finish(int acc, float sa, float sb, float bias,
   return gelu ? gelu_tanh(v) : v;
 }
 
+__device__ __forceinline__ uint32_t pack2(int out, float lo, float hi) {
+  uint32_t r;
+  if (out == kOutBF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 template <int OUT>
 __device__ __forceinline__ void store_one(void* C, long long at, int acc, float v) {
   if (OUT == kOutF32) ((float*)C)[at] = v;
-  else if (OUT == kOutBF16) ((__nv_bfloat16*)C)[at] = __float2bfloat16_rn(v);
-  else if (OUT == kOutF16) ((__half*)C)[at] = __float2half_rn(v);
-  else ((int*)C)[at] = acc;
+  else if (OUT == kOutS32) ((int*)C)[at] = acc;
+  else ((uint16_t*)C)[at] = (uint16_t)(pack2(OUT, v, 0.f) & 0xffffu);
 }
 
-// 64 x 64 tiles, 16 k at a time, 4 x 4 sums per thread, one byte per load: any size, pitch and address.
+// ---------------------------------------------------------------------------------------- one CTA per tile
+template <int BT>
+struct TileCfg {
+  static constexpr int kBBytes = 128 * BK;       // channels
+  static constexpr int kABytes = BT * BK;        // tokens
+  static constexpr int kStage = kABytes + kBBytes;
+  // about 100 KB, so that two CTAs share an SM and one's loads run under the other's end
+  static constexpr int kStages = BT == 32 ? 5 : BT == 64 ? 4 : 3;
+  static constexpr int kSmem = kStages * kStage + 1024 + 256;
+  static_assert(kStages * kStage >= BT * 128 * 4, "the sums of a tile lie over its stages");
+};
+
+// Shared memory of CTA `rank` of the cluster at this CTA's offset `p`.
+__device__ __forceinline__ int4 ld_cluster_v4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Tile of 128 channels x BT tokens; the cluster's `splits` CTAs take a slice of K each.
+template <int BT, int OUT>
+__global__ void __launch_bounds__(kThreads)
+gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, void* __restrict__ C,
+                    long long ldc, int M, int N, int K, int splits, const Epilogue ep, int vec_store) {
+  using CF = TileCfg<BT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = (uint64_t*)(smem + CF::kStages * CF::kStage);
+  uint64_t* empty = full + CF::kStages;
+  uint64_t* acc_full = empty + CF::kStages;
+  uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nb = (N + 127) / 128;
+  const int rank = (int)(blockIdx.x % splits), tile = (int)(blockIdx.x / splits);
+  const int n0 = (tile % nb) * 128, t0 = (tile / nb) * BT;
+  const int kbs = (K + BK - 1) / BK, kps = (kbs + splits - 1) / splits;
+  const int kb0 = rank * kps, kb1 = min(kbs, kb0 + kps);   // never empty (the host picks `splits` so)
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < CF::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, BT);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0, issued = 0, fill_par = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&empty[s], ph ^ 1, kErrTimeoutEmpty, &g_tc_error_gemm_i8)) break;
+        mbar_arrive_expect_tx(&full[s], CF::kStage);
+        uint8_t* st = smem + s * CF::kStage;
+        tma_load_2d_map(&tmB, &full[s], st, kb * BK, n0);
+        tma_load_2d_map(&tmA, &full[s], st + CF::kBBytes, kb * BK, t0);
+        issued |= 1u << s;
+        fill_par = (fill_par & ~(1u << s)) | (ph << s);
+        if (++s == CF::kStages) { s = 0; ph ^= 1; }
+      }
+      // never leave, nor lay the sums over a stage, with TMA writes in flight
+      for (int q = 0; q < CF::kStages; ++q)
+        if (issued & (1u << q)) mbar_wait(&full[q], (fill_par >> q) & 1, kErrTimeoutOther, &g_tc_error_gemm_i8);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_i8(128, BT);
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = mbar_wait(&full[s], ph, kErrTimeoutFull, &g_tc_error_gemm_i8);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t b_addr = smem_u32(smem + s * CF::kStage), a_addr = b_addr + CF::kBBytes;
+#pragma unroll
+        for (int k = 0; k < BK / 32; ++k)
+          mma_i8_ss(tmem, sw128_desc(b_addr + k * 32), sw128_desc(a_addr + k * 32), idesc, ((kb - kb0) | k) != 0);
+        mma_commit(&empty[s]);
+        if (++s == CF::kStages) { s = 0; ph ^= 1; }
+      }
+      if (ok) mma_commit(acc_full);
+    }
+  }
+  __syncwarp();
+  // the tile's sums, [token][channel], over the stages
+  int* sums = (int*)smem;
+  const bool done = mbar_wait_warp(acc_full, 0, kErrTimeoutAcc, &g_tc_error_gemm_i8);
+  __syncthreads();                               // the TMA thread has seen its last fill land
+  if (warp >= 2 && done) {
+    tc_fence_after();
+    const int q = warp & 3;                      // TMEM lane quarter this warp may access
+#pragma unroll
+    for (int c = 0; c < BT; c += 32) {
+      uint32_t v[32];
+      tmem_ld16(tmem + c + ((uint32_t)(q * 32) << 16), *reinterpret_cast<uint32_t(*)[16]>(v));
+      tmem_ld16(tmem + c + 16 + ((uint32_t)(q * 32) << 16), *reinterpret_cast<uint32_t(*)[16]>(v + 16));
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) sums[(c + j) * 128 + q * 32 + lane] = (int)v[j];
+    }
+    tc_fence_before();
+  }
+  if (splits > 1) cluster_sync();
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, BT);
+  }
+  // a warp per token: a lane adds and finishes four channels
+  const int per = (BT + splits - 1) / splits, j1 = min(min(BT, (rank + 1) * per), M - t0);
+  const int n = n0 + lane * 4;
+  float sb[4], bias[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    sb[e] = ep.b_scale && n + e < N ? ep.b_scale[n + e] : 1.f;
+    bias[e] = ep.bias && n + e < N ? ep.bias[n + e] : 0.f;
+  }
+  if (n < N) {
+    for (int j = rank * per + warp; j < j1; j += kThreads / 32) {
+      int4 acc = make_int4(0, 0, 0, 0);
+      const int* at = sums + j * 128 + lane * 4;
+      if (splits == 1) {
+        acc = *(const int4*)at;
+      } else {
+        for (int c = 0; c < splits; ++c) {
+          const int4 p = ld_cluster_v4(cluster_addr(at, c));
+          acc.x += p.x; acc.y += p.y; acc.z += p.z; acc.w += p.w;
+        }
+      }
+      const long long o = (long long)(t0 + j) * ldc + n;
+      const int a4[4] = {acc.x, acc.y, acc.z, acc.w};
+      float v[4] = {};
+      if (OUT != kOutS32) {
+        const float sa = ep.a_scale ? ep.a_scale[t0 + j] : 1.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = finish(a4[e], sa, sb[e], bias[e], ep.gelu);
+      }
+      if (vec_store && n + 4 <= N) {
+        if (OUT == kOutS32) *(int4*)((int*)C + o) = acc;
+        else if (OUT == kOutF32) *(float4*)((float*)C + o) = make_float4(v[0], v[1], v[2], v[3]);
+        else *(uint2*)((uint16_t*)C + o) = make_uint2(pack2(OUT, v[0], v[1]), pack2(OUT, v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < N) store_one<OUT>(C, o + e, a4[e], v[e]);
+      }
+    }
+  }
+  if (splits > 1) {
+    __syncwarp();
+    cluster_sync();                              // no CTA leaves while the others read its sums
+  }
+}
+
+// ---------------------------------------------------------------------------------------- CTA pairs
+struct PairCfg {
+  static constexpr int BN = 256;
+  static constexpr int kABytes = 128 * BK, kBBytes = BN / 2 * BK;
+  static constexpr int kStage = kABytes + kBBytes;
+  static constexpr int kStages = 6;
+  static constexpr int kBox = 4 * 4096;          // per epilogue warp: 32 rows x 128 bytes
+  static constexpr int kSmem = kStages * kStage + 1024 + 1024 + kBox;
+  static constexpr int kTmemCols = 2 * BN;
+};
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+               ::"l"(map), "r"(smem_u32(src)), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read0() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// Bands of kGroupM token blocks, channel blocks inside a band: tiles worked on at the same time share operand
+// blocks in L2.
+constexpr int kGroupM = 16;
+__device__ __forceinline__ void pair_tile(int t, int mb, int nb, int* m_blk, int* n_blk) {
+  const int band = t / (kGroupM * nb), first = band * kGroupM;
+  const int rows = min(mb - first, kGroupM);
+  const int q = t - band * kGroupM * nb;
+  *m_blk = first + q % rows;
+  *n_blk = q / rows;
+}
+
 template <int OUT>
-__global__ void __launch_bounds__(256) gemm_i8_simt_kernel(const int8_t* __restrict__ A, long long lda, const int8_t* __restrict__ B,
-                                                           long long ldb, void* __restrict__ C, long long ldc, int M, int N, int K,
-                                                           const Epilogue ep) {
-  __shared__ int As[64][5], Bs[64][5];           // 16 bytes a row, and a word apart from the next bank
-  const long long m0 = (long long)blockIdx.y * 64, n0 = (long long)blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < K; k0 += 16) {
-    for (int e = threadIdx.x; e < 64 * 16; e += 256) {
-      const int row = e >> 4, k = k0 + (e & 15);
-      ((int8_t*)As[row])[e & 15] = m0 + row < M && k < K ? A[(m0 + row) * lda + k] : (int8_t)0;
-      ((int8_t*)Bs[row])[e & 15] = n0 + row < N && k < K ? B[(n0 + row) * ldb + k] : (int8_t)0;
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmC, void* __restrict__ C, long long ldc, int M, int N, int K,
+                    const Epilogue ep, int tma_store) {
+  using CF = PairCfg;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = (uint64_t*)(smem + CF::kStages * CF::kStage);
+  uint64_t* empty = full + CF::kStages;
+  uint64_t* acc_full = empty + CF::kStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+  uint8_t* box_base = smem + CF::kStages * CF::kStage + 1024;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();          // the even CTA issues the MMAs
+  const int mb = (M + 255) / 256, nb = (N + CF::BN - 1) / CF::BN;
+  const int tiles = mb * nb, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int kbs = (K + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < CF::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(As[ty + 16 * i][w], Bs[tx + 16 * j][w], acc[i][j]);
-    __syncthreads();
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 256);             // the epilogue threads of both CTAs
+    }
+    fence_barrier_init();
   }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, CF::kTmemCols);
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tmap(&tmA);
+      prefetch_tmap(&tmB);
+      int s = 0;
+      uint32_t ph = 0, issued = 0, fill_par = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        int m_blk, n_blk;
+        pair_tile(t, mb, nb, &m_blk, &n_blk);
+        const int a_row = m_blk * 256 + (int)rank * 128, b_row = n_blk * CF::BN + (int)rank * (CF::BN / 2);
+        for (int kb = 0; kb < kbs; ++kb) {
+          ok = mbar_wait(&empty[s], ph ^ 1, kErrTimeoutEmpty, &g_tc_error_gemm_i8);
+          if (!ok) break;
+          // both CTAs' loads complete on the even CTA's barrier, armed there for both
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * CF::kStage);
+          const uint32_t bar = cluster_addr(&full[s], 0);
+          uint8_t* st = smem + s * CF::kStage;
+          tma_load_2d_pair(&tmA, bar, st, kb * BK, a_row);
+          tma_load_2d_pair(&tmB, bar, st + CF::kABytes, kb * BK, b_row);
+          issued |= 1u << s;
+          fill_par = (fill_par & ~(1u << s)) | (ph << s);
+          if (++s == CF::kStages) { s = 0; ph ^= 1; }
+        }
+      }
+      // never leave with TMA writes in flight (the odd CTA stays until the final cluster barrier, which the
+      // even CTA reaches after this wait for both CTAs' loads)
+      if (rank == 0)
+        for (int q = 0; q < CF::kStages; ++q)
+          if (issued & (1u << q)) mbar_wait(&full[q], (fill_par >> q) & 1, kErrTimeoutOther, &g_tc_error_gemm_i8);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = idesc_i8(256, CF::BN);
+      int s = 0, local = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs, ++local) {
+        const int a = local & 1;
+        if (!mbar_wait(&acc_empty[a], ((local >> 1) & 1) ^ 1, kErrTimeoutAccEmpty, &g_tc_error_gemm_i8)) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + a * CF::BN;
+        for (int kb = 0; kb < kbs; ++kb) {
+          ok = mbar_wait(&full[s], ph, kErrTimeoutFull, &g_tc_error_gemm_i8);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(smem + s * CF::kStage), b_addr = a_addr + CF::kABytes;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long m = m0 + ty + 16 * i;
-    if (m >= M) continue;
-    const float sa = ep.a_scale ? ep.a_scale[m] : 1.f;
+          for (int k = 0; k < BK / 32; ++k)
+            mma_i8_ss_pair(d, sw128_desc(a_addr + k * 32), sw128_desc(b_addr + k * 32), idesc, (kb | k) != 0);
+          mma_commit_pair(&empty[s]);            // frees the stage in both CTAs
+          if (++s == CF::kStages) { s = 0; ph ^= 1; }
+        }
+        if (ok) mma_commit_pair(&acc_full[a]);
+      }
+    }
+  } else {
+    const int q = warp & 3;                      // TMEM lane quarter this warp may access
+    uint8_t* box = box_base + (warp - 2) * 4096;
+    int local = 0;
+    for (int t = pair; t < tiles; t += pairs, ++local) {
+      const int a = local & 1;
+      if (!mbar_wait_warp(&acc_full[a], (local >> 1) & 1, kErrTimeoutAcc, &g_tc_error_gemm_i8)) break;
+      tc_fence_after();
+      int m_blk, n_blk;
+      pair_tile(t, mb, nb, &m_blk, &n_blk);
+      const int r0 = m_blk * 256 + (int)rank * 128 + q * 32, row = r0 + lane;   // this thread's token
+      const uint32_t taddr = tmem_base + a * CF::BN + ((uint32_t)(q * 32) << 16);
+      const float sa = ep.a_scale && row < M ? ep.a_scale[row] : 1.f;
+#pragma unroll 1
+      for (int c = 0; c < CF::BN; c += 32) {
+        const int col = n_blk * CF::BN + c;
+        if (col >= N) break;                     // warp-uniform
+        uint32_t v[32];
+        tmem_ld16(taddr + c, *reinterpret_cast<uint32_t(*)[16]>(v));
+        tmem_ld16(taddr + c + 16, *reinterpret_cast<uint32_t(*)[16]>(v + 16));
+        // lane l holds channel col + l's scale and bias, handed round by shuffles
+        const float sbl = ep.b_scale && col + lane < N ? ep.b_scale[col + lane] : 1.f;
+        const float bil = ep.bias && col + lane < N ? ep.bias[col + lane] : 0.f;
+        tmem_wait_ld();
+        if (OUT != kOutS32) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const long long n = n0 + tx + 16 * j;
-      if (n >= N) continue;
-      const float v = OUT == kOutS32 ? 0.f
-                                     : finish(acc[i][j], sa, ep.b_scale ? ep.b_scale[n] : 1.f, ep.bias ? ep.bias[n] : 0.f, ep.gelu);
-      store_one<OUT>(C, m * ldc + n, acc[i][j], v);
+          for (int j = 0; j < 32; ++j) {
+            const float sb = __shfl_sync(0xffffffffu, sbl, j), bi = __shfl_sync(0xffffffffu, bil, j);
+            v[j] = __float_as_uint(finish((int)v[j], sa, sb, bi, ep.gelu));
+          }
+        }
+        if (tma_store) {
+          // rows of 128 bytes in a swizzled box of 32 rows, one TMA store for 32 four-byte or 64 two-byte
+          // columns: whole lines, and the tensor map clips the tails
+          constexpr int kW = 32 * kOutBytes<OUT> / 4;                      // 4-byte words of this chunk's row
+          const int half = kW == 16 ? (c / 32) & 1 : 0;
+          uint32_t w[kW];
+#pragma unroll
+          for (int j = 0; j < kW; ++j)
+            w[j] = kW == 32 ? v[j] : pack2(OUT, __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+          if (half == 0) {
+            if (lane == 0) bulk_wait_read0();    // the previous store has read the box
+            __syncwarp();
+          }
+#pragma unroll
+          for (int i = 0; i < kW / 4; ++i)
+            *(uint4*)(box + lane * 128 + (((i + half * 4) ^ (lane & 7)) << 4)) =
+                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          if (kW == 32 || half == 1 || col + 32 >= N) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmC, box, kW == 32 ? col : col - half * 32, r0);
+              bulk_commit();
+            }
+          }
+        } else {
+          // rows of C that TMA cannot write: 32 x 32 results through shared memory, stored row by row
+          uint32_t* stage = (uint32_t*)box;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) stage[lane * 32 + (j ^ lane)] = v[j];
+          __syncwarp();
+#pragma unroll 4
+          for (int rr = 0; rr < 32; ++rr) {
+            const uint32_t x = stage[rr * 32 + (lane ^ rr)];
+            if (r0 + rr < M && col + lane < N) store_one<OUT>(C, (long long)(r0 + rr) * ldc + col + lane, (int)x, __uint_as_float(x));
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      if (rank == 0) mbar_arrive(&acc_empty[a]);
+      else mbar_arrive_remote(cluster_addr(&acc_empty[a], 0));
+    }
+    if (lane == 0) bulk_wait_all();              // the stores complete before the shared memory goes away
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();                                // neither CTA leaves while the pair's MMAs may read it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, CF::kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------------------- operands
+// Rows of `src` (any address and pitch) copied to 16-byte aligned rows `pitch` bytes apart, 16 bytes a thread;
+// both operands in one launch.  A word that holds a byte of the row is read whole.
+struct PackArgs {
+  const uint8_t* src[2];
+  uint8_t* dst[2];
+  long long ld[2], chunks[2];                    // chunks: 16-byte pieces of all rows (0: nothing to copy)
+  int K, per_row;
+};
+__global__ void __launch_bounds__(256) pack_rows_kernel(const PackArgs p) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < p.chunks[0] + p.chunks[1]; i += (long long)gridDim.x * 256) {
+    const int w = i >= p.chunks[0];
+    const long long e = w ? i - p.chunks[0] : i, row = e / p.per_row;
+    const int k = (int)(e % p.per_row) * 16;
+    const uint8_t* at = p.src[w] + row * p.ld[w] + k;
+    const int shift = (int)((uintptr_t)at & 3), left = p.K - k;   // bytes of the row from here on
+    const uint32_t* words = (const uint32_t*)(at - shift);
+    uint32_t x[5];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) x[j] = 4 * j < left + shift ? words[j] : 0u;
+    uint32_t y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = __funnelshift_r(x[j], x[j + 1], 8 * shift);
+    *(uint4*)(p.dst[w] + row * (long long)p.per_row * 16 + k) = make_uint4(y[0], y[1], y[2], y[3]);
+  }
+}
+
+// K = 0: every sum is 0.
+template <int OUT>
+__global__ void __launch_bounds__(256) no_depth_kernel(void* __restrict__ C, long long ldc, int M, int N, const Epilogue ep) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)M * N; i += (long long)gridDim.x * 256) {
+    const long long m = i / N, n = i % N;
+    const float v = OUT == kOutS32 ? 0.f
+                                   : finish(0, ep.a_scale ? ep.a_scale[m] : 1.f, ep.b_scale ? ep.b_scale[n] : 1.f,
+                                            ep.bias ? ep.bias[n] : 0.f, ep.gelu);
+    store_one<OUT>(C, m * ldc + n, 0, v);
+  }
+}
+
+bool TmaRows(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 16 == 0; }
+int64_t PackedPitch(int64_t K) { return (K + 15) / 16 * 16; }
+size_t PackedBytes(const void* p, int64_t ld, int64_t rows, int64_t K) {
+  return TmaRows(p, ld) ? 0 : ((size_t)rows * PackedPitch(K) + 255) / 256 * 256;
+}
+
+// 2-D map over [rows, K] bytes, `box_rows` rows of one 128-byte swizzle row.
+bool MakeI8Map(CUtensorMap* map, const void* p, int64_t ld, int rows, int K, int box_rows) {
+  EncodeTiledFn enc = GetEncodeTiled();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {BK, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// 2-D map over C for the pair kernel's stores: boxes of 32 rows x 128 bytes, 128-byte swizzle.
+bool MakeOutMap(CUtensorMap* map, void* C, int64_t ldc, int M, int N, int out) {
+  EncodeTiledFn enc = GetEncodeTiled();
+  if (!enc) return false;
+  const int es = out == kOutBF16 || out == kOutF16 ? 2 : 4;
+  cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
+  cuuint64_t strides[1] = {(cuuint64_t)ldc * es};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / es), 32}, estr[2] = {1, 1};
+  const CUtensorMapDataType t = out == kOutF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                              : out == kOutS32 ? CU_TENSOR_MAP_DATA_TYPE_INT32
+                              : out == kOutBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(map, t, 2, C, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Call {
+  const void* A;
+  const void* B;
+  void* C;
+  int64_t lda, ldb, ldc;
+  int M, N, K, out;
+  Epilogue ep;
+  cudaStream_t st;
+};
+
+// The launch form of a product: CTA pairs, or single tiles of `bt` tokens with K cut over `splits` CTAs.
+struct Form {
+  bool pair = false;
+  int bt = 32, splits = 1;
+};
+
+int Launched(cudaError_t e) {
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return -3;
+  }
+  CountLaunches();
+  return 0;
+}
+
+// Whether `kernel` may use `smem` bytes on the current device; asked of the driver once for each of 64 devices.
+template <typename Kernel>
+cudaError_t AllowSmem(Kernel* kernel, int smem, std::atomic<uint64_t>* known) {
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (known->load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
+  known->fetch_or(bit, std::memory_order_relaxed);
+  return cudaSuccess;
+}
+
+template <typename Kernel, typename... Args>
+int LaunchClusters(Kernel* kernel, int grid, int cluster, int smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return Launched(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
+template <int BT, int OUT>
+int LaunchTile(const Call& c, int splits) {
+  CUtensorMap ta, tb;
+  if (!MakeI8Map(&ta, c.A, c.lda, c.M, c.K, BT) || !MakeI8Map(&tb, c.B, c.ldb, c.N, c.K, 128)) return -2;
+  const int64_t grid = (int64_t)((c.N + 127) / 128) * ((c.M + BT - 1) / BT) * splits;
+  if (grid > INT32_MAX) return -1;
+  const int lane_bytes = 4 * kOutBytes<OUT>;     // a lane's four channels
+  const int vec = (uintptr_t)c.C % lane_bytes == 0 && c.ldc % 4 == 0;
+  static std::atomic<uint64_t> known{0};
+  if (cudaError_t e = AllowSmem(gemm_i8_tile_kernel<BT, OUT>, TileCfg<BT>::kSmem, &known)) return Launched(e);
+  return LaunchClusters(gemm_i8_tile_kernel<BT, OUT>, (int)grid, splits, TileCfg<BT>::kSmem, c.st, ta, tb, c.C, (long long)c.ldc,
+                        c.M, c.N, c.K, splits, c.ep, vec);
+}
+
+template <int OUT>
+int LaunchPair(const Call& c) {
+  CUtensorMap ta, tb, tc;
+  if (!MakeI8Map(&ta, c.A, c.lda, c.M, c.K, 128) || !MakeI8Map(&tb, c.B, c.ldb, c.N, c.K, 128)) return -2;
+  const int tma_store = (uintptr_t)c.C % 16 == 0 && c.ldc * kOutBytes<OUT> % 16 == 0 && MakeOutMap(&tc, c.C, c.ldc, c.M, c.N, OUT);
+  if (!tma_store) tc = ta;                       // unused
+  const int64_t tiles = (int64_t)((c.M + 255) / 256) * ((c.N + 255) / 256);
+  if (tiles > INT32_MAX / 2) return -1;
+  static std::atomic<uint64_t> known{0};
+  if (cudaError_t e = AllowSmem(gemm_i8_pair_kernel<OUT>, PairCfg::kSmem, &known)) return Launched(e);
+  const int pairs = (int)std::min<int64_t>(tiles, NumSMs() / 2);   // one CTA per SM
+  return LaunchClusters(gemm_i8_pair_kernel<OUT>, 2 * pairs, 2, PairCfg::kSmem, c.st, ta, tb, tc, c.C, (long long)c.ldc, c.M, c.N,
+                        c.K, c.ep, tma_store);
+}
+
+template <int OUT>
+int LaunchNoDepth(const Call& c) {
+  const int64_t n = (int64_t)c.M * c.N;
+  no_depth_kernel<OUT><<<(unsigned)std::min<int64_t>((n + 255) / 256, NumSMs() * 8), 256, 0, c.st>>>(c.C, c.ldc, c.M, c.N, c.ep);
+  return Launched(cudaGetLastError());
+}
+
+template <int OUT>
+int LaunchForm(const Call& c, const Form& f) {
+  if (c.K == 0) return LaunchNoDepth<OUT>(c);
+  if (f.pair) return LaunchPair<OUT>(c);
+  if (f.bt == 32) return LaunchTile<32, OUT>(c, f.splits);
+  if (f.bt == 64) return LaunchTile<64, OUT>(c, f.splits);
+  return LaunchTile<128, OUT>(c, f.splits);
+}
+
+Form ChooseForm(int64_t M, int64_t N, int64_t K, int sms) {
+  Form f;
+  f.bt = M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  const int64_t kbs = (K + BK - 1) / BK;
+  const int64_t tiles = ((N + 127) / 128) * ((M + f.bt - 1) / f.bt);
+  const int64_t pair_tiles = ((M + 255) / 256) * ((N + 255) / 256);
+  f.pair = M >= 256 && pair_tiles * 2 >= sms;
+  for (int s = 8; s > 1; s /= 2) {
+    const int64_t kps = (kbs + s - 1) / s;
+    if (tiles * s <= 2 * sms && kps >= 2 && (s - 1) * kps < kbs) {
+      f.splits = s;
+      break;
     }
   }
+  // B200_GEMM_I8_FORM = pair, or <tokens>x<splits>: every product in that form (for comparisons)
+  if (const char* env = std::getenv("B200_GEMM_I8_FORM")) {
+    int bt = 0, s = 0;
+    f.pair = env[0] == 'p';
+    if (!f.pair && std::sscanf(env, "%dx%d", &bt, &s) == 2 && (bt == 32 || bt == 64 || bt == 128) && s >= 1 && s <= 8) {
+      f.bt = bt;
+      for (f.splits = s; f.splits > 1; --f.splits)
+        if ((f.splits - 1) * ((kbs + f.splits - 1) / f.splits) < kbs) break;
+    }
+  }
+  return f;
 }
 
 int OutCodeI8(int type) {
@@ -90,28 +653,61 @@ int OutCodeI8(int type) {
 
 }  // namespace
 
-size_t GemmI8ScratchBytes(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K) { return 0; }
+int TakeGemmI8Error() {
+  int v = 0, z = 0;
+  cudaMemcpyFromSymbol(&v, g_tc_error_gemm_i8, sizeof(int));
+  if (v) cudaMemcpyToSymbol(g_tc_error_gemm_i8, &z, sizeof(int));
+  return v;
+}
+
+size_t GemmI8ScratchBytes(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return PackedBytes(A, lda, M, K) + PackedBytes(B, ldb, N, K);
+}
 
 int GemmI8(const void* A, int64_t lda, const void* B, int64_t ldb, const float* a_scale, const float* b_scale, const float* bias,
            void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, int out_type, int act, void* scratch, size_t scratch_bytes,
            cudaStream_t st) {
   const int out = OutCodeI8(out_type);
-  if (out < 0 || M < 0 || N < 0 || K < 0 || M > INT32_MAX || N > INT32_MAX || K > kGemmI8MaxK || lda < K || ldb < K || ldc < N)
+  if (out < 0 || M < 0 || N < 0 || K < 0 || M > INT32_MAX - 256 || N > INT32_MAX - 256 || K > kGemmI8MaxK || lda < K || ldb < K ||
+      ldc < N)
     return -1;
-  if (act < 0 || act > 1 || (out == kOutS32 && (a_scale || b_scale || bias || act))) return -1;
+  if (act < B200_ACT_NONE || act > B200_ACT_GELU || (out == kOutS32 && (a_scale || b_scale || bias || act))) return -1;
   if (M == 0 || N == 0) return 0;
   const int es = out == kOutBF16 || out == kOutF16 ? 2 : 4;
   if ((K && (!A || !B)) || !C || (uintptr_t)C % es || (uintptr_t)a_scale % 4 || (uintptr_t)b_scale % 4 || (uintptr_t)bias % 4) return -1;
-  if ((M + 63) / 64 > 65535) return -1;
-  const Epilogue ep = {a_scale, b_scale, bias, act};
-  const dim3 grid((unsigned)((N + 63) / 64), (unsigned)((M + 63) / 64));
-  const int8_t *a = (const int8_t*)A, *b = (const int8_t*)B;
-  if (out == kOutF32) gemm_i8_simt_kernel<kOutF32><<<grid, 256, 0, st>>>(a, lda, b, ldb, C, ldc, (int)M, (int)N, (int)K, ep);
-  else if (out == kOutBF16) gemm_i8_simt_kernel<kOutBF16><<<grid, 256, 0, st>>>(a, lda, b, ldb, C, ldc, (int)M, (int)N, (int)K, ep);
-  else if (out == kOutF16) gemm_i8_simt_kernel<kOutF16><<<grid, 256, 0, st>>>(a, lda, b, ldb, C, ldc, (int)M, (int)N, (int)K, ep);
-  else gemm_i8_simt_kernel<kOutS32><<<grid, 256, 0, st>>>(a, lda, b, ldb, C, ldc, (int)M, (int)N, (int)K, ep);
-  CountLaunches();
-  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+  const size_t need_a = K ? PackedBytes(A, lda, M, K) : 0, need_b = K ? PackedBytes(B, ldb, N, K) : 0;
+  if (need_a + need_b && (!scratch || need_a + need_b > scratch_bytes || (uintptr_t)scratch % 256)) return -4;
+  Call c = {A, B, C, lda, ldb, ldc, (int)M, (int)N, (int)K, out, {a_scale, b_scale, bias, act}, st};
+  if (need_a + need_b) {
+    PackArgs p = {};
+    p.K = c.K;
+    p.per_row = (int)(PackedPitch(K) / 16);
+    if (need_a) {
+      p.src[0] = (const uint8_t*)A;
+      p.dst[0] = (uint8_t*)scratch;
+      p.ld[0] = lda;
+      p.chunks[0] = M * p.per_row;
+      c.A = p.dst[0];
+      c.lda = PackedPitch(K);
+    }
+    if (need_b) {
+      p.src[1] = (const uint8_t*)B;
+      p.dst[1] = (uint8_t*)scratch + need_a;
+      p.ld[1] = ldb;
+      p.chunks[1] = N * p.per_row;
+      c.B = p.dst[1];
+      c.ldb = PackedPitch(K);
+    }
+    const long long blocks = (p.chunks[0] + p.chunks[1] + 255) / 256;
+    pack_rows_kernel<<<(unsigned)std::min<long long>(blocks, NumSMs() * 16), 256, 0, st>>>(p);
+    if (int rc = Launched(cudaGetLastError())) return rc;
+  }
+  const Form f = ChooseForm(M, N, K, NumSMs());
+  if (out == kOutF32) return LaunchForm<kOutF32>(c, f);
+  if (out == kOutBF16) return LaunchForm<kOutBF16>(c, f);
+  if (out == kOutF16) return LaunchForm<kOutF16>(c, f);
+  return LaunchForm<kOutS32>(c, f);
 }
 
 }  // namespace b200k

@@ -76,6 +76,7 @@ int AttentionBwd(const void* q, const void* k, const void* v, const void* o, con
 
 // ---- device error flags of the bounded waits ----------------------------------------------------
 int TakeGemmError();
+int TakeGemmI8Error();
 int TakeAttnError();
 int TakeAttnBwdError();
 

@@ -57,6 +57,20 @@ def test_gemm_refusals(k, change):
     refused(lambda: k.gemm_i8(**{**a, **change}))
 
 
+@pytest.mark.parametrize("change,need", [({}, 0), (dict(a=P + 1), 8 * 48), (dict(lda=33), 8 * 48), (dict(b=P + 8), 16 * 48),
+                                         (dict(lda=33, ldb=34), 24 * 48)])
+def test_gemm_scratch(k, change, need):
+    """Operands that do not lie 16-byte aligned need room for copies, each rounded up to 256 bytes."""
+    a = {**dict(a=P, lda=48, b=P, ldb=48, m=8, n=16, k=33), **change}
+    room = sum((r * 48 + 255) // 256 * 256 for r, moved in ((8, a["a"] % 16 or a["lda"] % 16), (16, a["b"] % 16 or a["ldb"] % 16)) if moved)
+    assert k.gemm_i8_scratch_bytes(**a) == room >= need
+    if room:
+        call = dict(a_scale=None, b_scale=None, bias=None, c=P, ldc=16, out_type=BF16)
+        refused(lambda: k.gemm_i8(**a, **call), -4)
+        refused(lambda: k.gemm_i8(**a, **call, scratch=P, scratch_bytes=room - 1), -4)
+        refused(lambda: k.gemm_i8(**a, **call, scratch=P + 16, scratch_bytes=room + 256), -4)
+
+
 def test_empty_calls_do_nothing(k):
     k.quantize_i8(None, 16, None, 16, None, 0, 16, BF16)
     k.rms_norm_i8(None, 16, None, 0, None, None, 0, None, 16, None, 0, 16, BF16, F32, 1e-5)
@@ -267,6 +281,34 @@ def test_gemm_sums(k, cuda, m, n, kk, pad, offset):
     kept = flat.clone()
     kept[offset:offset + m * (n + pad)].view(m, n + pad)[:, :n] = 123456789
     assert bool((kept == 123456789).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["pair", "32x1", "32x3", "32x8", "64x1", "64x4", "64x7", "128x1", "128x2", "128x5", "128x8"])
+@pytest.mark.parametrize("m,n,kk", [(1, 300, 1500), (70, 130, 1024), (300, 520, 1000), (515, 1031, 1280)])
+@pytest.mark.parametrize("npad", [0, 3])
+def test_gemm_every_form(k, cuda, monkeypatch, form, m, n, kk, npad):
+    """CTA pairs, and single tiles of 32 to 128 tokens with K cut over up to 8 CTAs, whatever the size."""
+    torch = cuda
+    monkeypatch.setenv("B200_GEMM_I8_FORM", form)
+    g = torch.Generator(device="cuda").manual_seed(m + n + kk)
+    a, b = operand(torch, g, m, kk, 0), operand(torch, g, n, kk, 0)
+    s, size = scratch_for(torch, k, a, kk, b, kk, m, n, kk)
+    sa, sb = torch.rand(m, device="cuda", generator=g) * 0.01, torch.rand(n, device="cuda", generator=g) * 0.01
+    bias = torch.randn(n, device="cuda", generator=g)
+    for out_type in (S32, F32, BF16, F16):
+        dtype = torch.int32 if out_type == S32 else types(torch)[out_type]
+        c, flat = rows_of(torch, m, n, npad, dtype, fill=99)
+        ptrs = [None] * 3 if out_type == S32 else [t.data_ptr() for t in (sa, sb, bias)]
+        k.gemm_i8(a.data_ptr(), kk, b.data_ptr(), kk, *ptrs, c.data_ptr(), n + npad, m, n, kk, out_type, 0, s.data_ptr(), size,
+                  stream(torch))
+        if out_type == S32:
+            assert torch.equal(c.double(), a.double() @ b.double().t())
+        else:
+            check_gemm(torch, c, *gemm_reference(torch, a, b, sa, sb, bias, False), out_type, False)
+        kept = flat.clone()
+        kept[:m * (n + npad)].view(m, n + npad)[:, :n] = 99
+        assert bool((kept == 99).all())
 
 
 def gemm_reference(torch, a, b, sa, sb, bias, gelu):
