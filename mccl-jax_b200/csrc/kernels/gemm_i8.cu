@@ -51,17 +51,55 @@ struct Epilogue {
   int gelu;
 };
 
+// Two f32 operations in one instruction.
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ uint64_t bits(F2 v) { return (uint64_t)__float_as_uint(v.y) << 32 | __float_as_uint(v.x); }
+__device__ __forceinline__ F2 floats(uint64_t b) { return {__uint_as_float((uint32_t)b), __uint_as_float((uint32_t)(b >> 32))}; }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+  return floats(d);
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+  return floats(d);
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return floats(d);
+}
+
+// Two integers as f32, rounded to nearest, without the conversion unit (a quarter of the rate and shared with
+// GELU's exponentials).  With H and L the halves of v + 2^31, the patterns 0x5300HHHH and 0x4b00LLLL are the
+// floats 2^39 + 2^16 H and 2^23 + L; taking 2^39 + 2^31 + 2^23 from the first is exact, and adding the second
+// rounds once.
+__device__ __forceinline__ F2 to_f32x2(int a, int b) {
+  constexpr float kOff = -(549755813888.f + 2147483648.f + 8388608.f);
+  const uint32_t u = (uint32_t)a ^ 0x80000000u, w = (uint32_t)b ^ 0x80000000u;
+  const F2 hi = {__uint_as_float(__byte_perm(u, 0x53000000u, 0x7632)), __uint_as_float(__byte_perm(w, 0x53000000u, 0x7632))};
+  const F2 lo = {__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7610)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7610))};
+  return add2(add2(hi, {kOff, kOff}), lo);
+}
+
 // The tanh form of GELU, 0.5 v (1 + tanh u) with u = sqrt(2 / pi) (v + 0.044715 v^3), as v / (1 + e^-2u):
 // the same function without the cancellation in 1 + tanh(u) for u < 0.
 __device__ __forceinline__ float gelu_tanh(float v) {
   constexpr float kU = -2.0f * 0.7978845608028654f * 1.4426950408889634f;   // -2 sqrt(2 / pi) log2(e)
-  const float e = exp2f(kU * v * fmaf(0.044715f * v, v, 1.0f));
-  return __fdividef(v, 1.0f + e);
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(kU * v * fmaf(0.044715f * v, v, 1.0f)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return v * r;
 }
 
-__device__ __forceinline__ float finish(int acc, float sa, float sb, float bias, int gelu) {
-  const float v = fmaf((float)acc * sa, sb, bias);
-  return gelu ? gelu_tanh(v) : v;
+// act(f32(acc) * sa * sb + bias) of two sums.
+__device__ __forceinline__ F2 finish2(int a, int b, float sa, F2 sb, F2 bias, int gelu) {
+  F2 v = fma2(mul2(to_f32x2(a, b), {sa, sa}), sb, bias);
+  if (gelu) v = {gelu_tanh(v.x), gelu_tanh(v.y)};
+  return v;
 }
 
 __device__ __forceinline__ uint32_t pack2(int out, float lo, float hi) {
@@ -86,7 +124,7 @@ struct TileCfg {
   static constexpr int kStage = kABytes + kBBytes;
   // about 100 KB, so that two CTAs share an SM and one's loads run under the other's end
   static constexpr int kStages = BT == 32 ? 5 : BT == 64 ? 4 : 3;
-  static constexpr int kSmem = kStages * kStage + 1024 + 256;
+  static constexpr int kSmem = kStages * kStage + 1024 + 256 + BT * 4;
   static_assert(kStages * kStage >= BT * 128 * 4, "the sums of a tile lie over its stages");
 };
 
@@ -109,6 +147,7 @@ gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   uint64_t* empty = full + CF::kStages;
   uint64_t* acc_full = empty + CF::kStages;
   uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
+  float* sa_of = (float*)(smem + CF::kStages * CF::kStage + 256);   // the tile's token scales
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nb = (N + 127) / 128;
   const int rank = (int)(blockIdx.x % splits), tile = (int)(blockIdx.x / splits);
@@ -129,6 +168,18 @@ gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+
+  // while the loads run: the scales and bias of this lane's four channels, and the tokens' scales
+  const int n = n0 + lane * 4;
+  F2 sb[2], bias[2];
+  auto channel = [&](const float* p, int j, float none) { return p && j < N ? p[j] : none; };
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    sb[e] = {channel(ep.b_scale, n + 2 * e, 1.f), channel(ep.b_scale, n + 2 * e + 1, 1.f)};
+    bias[e] = {channel(ep.bias, n + 2 * e, 0.f), channel(ep.bias, n + 2 * e + 1, 0.f)};
+  }
+  if (warp >= 2)
+    for (int j = threadIdx.x - 64; j < BT; j += kThreads - 64) sa_of[j] = ep.a_scale && t0 + j < M ? ep.a_scale[t0 + j] : 1.f;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -195,14 +246,8 @@ gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
   // a warp per token: a lane adds and finishes four channels
   const int per = (BT + splits - 1) / splits, j1 = min(min(BT, (rank + 1) * per), M - t0);
-  const int n = n0 + lane * 4;
-  float sb[4], bias[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    sb[e] = ep.b_scale && n + e < N ? ep.b_scale[n + e] : 1.f;
-    bias[e] = ep.bias && n + e < N ? ep.bias[n + e] : 0.f;
-  }
   if (n < N) {
+#pragma unroll 4
     for (int j = rank * per + warp; j < j1; j += kThreads / 32) {
       int4 acc = make_int4(0, 0, 0, 0);
       const int* at = sums + j * 128 + lane * 4;
@@ -215,21 +260,21 @@ gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
       }
       const long long o = (long long)(t0 + j) * ldc + n;
-      const int a4[4] = {acc.x, acc.y, acc.z, acc.w};
-      float v[4] = {};
+      F2 v[2] = {};
       if (OUT != kOutS32) {
-        const float sa = ep.a_scale ? ep.a_scale[t0 + j] : 1.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = finish(a4[e], sa, sb[e], bias[e], ep.gelu);
+        v[0] = finish2(acc.x, acc.y, sa_of[j], sb[0], bias[0], ep.gelu);
+        v[1] = finish2(acc.z, acc.w, sa_of[j], sb[1], bias[1], ep.gelu);
       }
       if (vec_store && n + 4 <= N) {
         if (OUT == kOutS32) *(int4*)((int*)C + o) = acc;
-        else if (OUT == kOutF32) *(float4*)((float*)C + o) = make_float4(v[0], v[1], v[2], v[3]);
-        else *(uint2*)((uint16_t*)C + o) = make_uint2(pack2(OUT, v[0], v[1]), pack2(OUT, v[2], v[3]));
+        else if (OUT == kOutF32) *(float4*)((float*)C + o) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        else *(uint2*)((uint16_t*)C + o) = make_uint2(pack2(OUT, v[0].x, v[0].y), pack2(OUT, v[1].x, v[1].y));
       } else {
+        const int a4[4] = {acc.x, acc.y, acc.z, acc.w};
+        const float v4[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (n + e < N) store_one<OUT>(C, o + e, a4[e], v[e]);
+          if (n + e < N) store_one<OUT>(C, o + e, a4[e], v4[e]);
       }
     }
   }
@@ -244,9 +289,11 @@ struct PairCfg {
   static constexpr int BN = 256;
   static constexpr int kABytes = 128 * BK, kBBytes = BN / 2 * BK;
   static constexpr int kStage = kABytes + kBBytes;
-  static constexpr int kStages = 6;
-  static constexpr int kBox = 4 * 4096;          // per epilogue warp: 32 rows x 128 bytes
-  static constexpr int kSmem = kStages * kStage + 1024 + 1024 + kBox;
+  static constexpr int kStages = 5;
+  static constexpr int kThreads = 64 + 256;      // TMA warp, MMA warp, eight epilogue warps
+  static constexpr int kBox = 8 * 4096;          // per epilogue warp: 32 rows x 128 bytes
+  static constexpr int kScales = 2 * 2 * BN * 4; // the tile's channel scales and biases, of two tiles in turn
+  static constexpr int kSmem = kStages * kStage + 1024 + 1024 + kBox + kScales;
   static constexpr int kTmemCols = 2 * BN;
 };
 
@@ -271,8 +318,8 @@ __device__ __forceinline__ void pair_tile(int t, int mb, int nb, int* m_blk, int
   *n_blk = q / rows;
 }
 
-template <int OUT>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int OUT, bool GELU>
+__global__ void __launch_bounds__(PairCfg::kThreads, 1)
 gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, void* __restrict__ C, long long ldc, int M, int N, int K,
                     const Epilogue ep, int tma_store) {
@@ -299,7 +346,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 256);             // the epilogue threads of both CTAs
+      mbar_init(&acc_empty[a], 512);             // the epilogue threads of both CTAs
     }
     fence_barrier_init();
   }
@@ -366,58 +413,75 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       }
     }
   } else {
-    const int q = warp & 3;                      // TMEM lane quarter this warp may access
+    // A warp reads its quarter of the tile's rows and one half of its columns.  The quarter follows from the
+    // warp's number: it may access 32 of the 128 lanes of tensor memory.
+    const int q = warp & 3, half = (warp - 2) >> 2;
     uint8_t* box = box_base + (warp - 2) * 4096;
+    float* scales = (float*)(box_base + CF::kBox);
     int local = 0;
+    bool ok = true;
     for (int t = pair; t < tiles; t += pairs, ++local) {
       const int a = local & 1;
-      if (!mbar_wait_warp(&acc_full[a], (local >> 1) & 1, kErrTimeoutAcc, &g_tc_error_gemm_i8)) break;
-      tc_fence_after();
       int m_blk, n_blk;
       pair_tile(t, mb, nb, &m_blk, &n_blk);
       const int r0 = m_blk * 256 + (int)rank * 128 + q * 32, row = r0 + lane;   // this thread's token
-      const uint32_t taddr = tmem_base + a * CF::BN + ((uint32_t)(q * 32) << 16);
+      float* sb_of = scales + a * 2 * CF::BN;
+      float* bias_of = sb_of + CF::BN;
       const float sa = ep.a_scale && row < M ? ep.a_scale[row] : 1.f;
+      {
+        const int j = threadIdx.x - 64, col = n_blk * CF::BN + j;
+        sb_of[j] = ep.b_scale && col < N ? ep.b_scale[col] : 1.f;
+        bias_of[j] = ep.bias && col < N ? ep.bias[col] : 0.f;
+      }
+      // the eight warps' values are there; and, as every warp is past the tile before, its half may be
+      // written again for the next.  A wait that gave up does not leave the loop: the others count on it here.
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      ok = ok && mbar_wait_warp(&acc_full[a], (local >> 1) & 1, kErrTimeoutAcc, &g_tc_error_gemm_i8);
+      if (!ok) continue;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + a * CF::BN + ((uint32_t)(q * 32) << 16);
 #pragma unroll 1
-      for (int c = 0; c < CF::BN; c += 32) {
+      for (int c = half * (CF::BN / 2); c < (half + 1) * (CF::BN / 2); c += 32) {
         const int col = n_blk * CF::BN + c;
         if (col >= N) break;                     // warp-uniform
         uint32_t v[32];
         tmem_ld16(taddr + c, *reinterpret_cast<uint32_t(*)[16]>(v));
         tmem_ld16(taddr + c + 16, *reinterpret_cast<uint32_t(*)[16]>(v + 16));
-        // lane l holds channel col + l's scale and bias, handed round by shuffles
-        const float sbl = ep.b_scale && col + lane < N ? ep.b_scale[col + lane] : 1.f;
-        const float bil = ep.bias && col + lane < N ? ep.bias[col + lane] : 0.f;
         tmem_wait_ld();
         if (OUT != kOutS32) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float sb = __shfl_sync(0xffffffffu, sbl, j), bi = __shfl_sync(0xffffffffu, bil, j);
-            v[j] = __float_as_uint(finish((int)v[j], sa, sb, bi, ep.gelu));
+          for (int j = 0; j < 32; j += 4) {
+            const float4 sb = *(const float4*)(sb_of + c + j), bi = *(const float4*)(bias_of + c + j);
+            const F2 lo = finish2((int)v[j], (int)v[j + 1], sa, {sb.x, sb.y}, {bi.x, bi.y}, GELU);
+            const F2 hi = finish2((int)v[j + 2], (int)v[j + 3], sa, {sb.z, sb.w}, {bi.z, bi.w}, GELU);
+            v[j] = __float_as_uint(lo.x);
+            v[j + 1] = __float_as_uint(lo.y);
+            v[j + 2] = __float_as_uint(hi.x);
+            v[j + 3] = __float_as_uint(hi.y);
           }
         }
         if (tma_store) {
           // rows of 128 bytes in a swizzled box of 32 rows, one TMA store for 32 four-byte or 64 two-byte
           // columns: whole lines, and the tensor map clips the tails
           constexpr int kW = 32 * kOutBytes<OUT> / 4;                      // 4-byte words of this chunk's row
-          const int half = kW == 16 ? (c / 32) & 1 : 0;
+          const int part = kW == 16 ? (c / 32) & 1 : 0;
           uint32_t w[kW];
 #pragma unroll
           for (int j = 0; j < kW; ++j)
             w[j] = kW == 32 ? v[j] : pack2(OUT, __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-          if (half == 0) {
+          if (part == 0) {
             if (lane == 0) bulk_wait_read0();    // the previous store has read the box
             __syncwarp();
           }
 #pragma unroll
           for (int i = 0; i < kW / 4; ++i)
-            *(uint4*)(box + lane * 128 + (((i + half * 4) ^ (lane & 7)) << 4)) =
+            *(uint4*)(box + lane * 128 + (((i + part * 4) ^ (lane & 7)) << 4)) =
                 make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-          if (kW == 32 || half == 1 || col + 32 >= N) {
+          if (kW == 32 || part == 1 || col + 32 >= N) {
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_2d(&tmC, box, kW == 32 ? col : col - half * 32, r0);
+              tma_store_2d(&tmC, box, col - part * 32, r0);
               bulk_commit();
             }
           }
@@ -482,10 +546,8 @@ template <int OUT>
 __global__ void __launch_bounds__(256) no_depth_kernel(void* __restrict__ C, long long ldc, int M, int N, const Epilogue ep) {
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)M * N; i += (long long)gridDim.x * 256) {
     const long long m = i / N, n = i % N;
-    const float v = OUT == kOutS32 ? 0.f
-                                   : finish(0, ep.a_scale ? ep.a_scale[m] : 1.f, ep.b_scale ? ep.b_scale[n] : 1.f,
-                                            ep.bias ? ep.bias[n] : 0.f, ep.gelu);
-    store_one<OUT>(C, m * ldc + n, 0, v);
+    const float sb = ep.b_scale ? ep.b_scale[n] : 1.f, bias = ep.bias ? ep.bias[n] : 0.f;
+    store_one<OUT>(C, m * ldc + n, 0, finish2(0, 0, ep.a_scale ? ep.a_scale[m] : 1.f, {sb, sb}, {bias, bias}, ep.gelu).x);
   }
 }
 
@@ -559,7 +621,7 @@ cudaError_t AllowSmem(Kernel* kernel, int smem, std::atomic<uint64_t>* known) {
 }
 
 template <typename Kernel, typename... Args>
-int LaunchClusters(Kernel* kernel, int grid, int cluster, int smem, cudaStream_t st, Args... args) {
+int LaunchClusters(Kernel* kernel, int grid, int threads, int cluster, int smem, cudaStream_t st, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -567,7 +629,7 @@ int LaunchClusters(Kernel* kernel, int grid, int cluster, int smem, cudaStream_t
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
@@ -585,11 +647,11 @@ int LaunchTile(const Call& c, int splits) {
   const int vec = (uintptr_t)c.C % lane_bytes == 0 && c.ldc % 4 == 0;
   static std::atomic<uint64_t> known{0};
   if (cudaError_t e = AllowSmem(gemm_i8_tile_kernel<BT, OUT>, TileCfg<BT>::kSmem, &known)) return Launched(e);
-  return LaunchClusters(gemm_i8_tile_kernel<BT, OUT>, (int)grid, splits, TileCfg<BT>::kSmem, c.st, ta, tb, c.C, (long long)c.ldc,
+  return LaunchClusters(gemm_i8_tile_kernel<BT, OUT>, (int)grid, kThreads, splits, TileCfg<BT>::kSmem, c.st, ta, tb, c.C, (long long)c.ldc,
                         c.M, c.N, c.K, splits, c.ep, vec);
 }
 
-template <int OUT>
+template <int OUT, bool GELU>
 int LaunchPair(const Call& c) {
   CUtensorMap ta, tb, tc;
   if (!MakeI8Map(&ta, c.A, c.lda, c.M, c.K, 128) || !MakeI8Map(&tb, c.B, c.ldb, c.N, c.K, 128)) return -2;
@@ -598,9 +660,9 @@ int LaunchPair(const Call& c) {
   const int64_t tiles = (int64_t)((c.M + 255) / 256) * ((c.N + 255) / 256);
   if (tiles > INT32_MAX / 2) return -1;
   static std::atomic<uint64_t> known{0};
-  if (cudaError_t e = AllowSmem(gemm_i8_pair_kernel<OUT>, PairCfg::kSmem, &known)) return Launched(e);
+  if (cudaError_t e = AllowSmem(gemm_i8_pair_kernel<OUT, GELU>, PairCfg::kSmem, &known)) return Launched(e);
   const int pairs = (int)std::min<int64_t>(tiles, NumSMs() / 2);   // one CTA per SM
-  return LaunchClusters(gemm_i8_pair_kernel<OUT>, 2 * pairs, 2, PairCfg::kSmem, c.st, ta, tb, tc, c.C, (long long)c.ldc, c.M, c.N,
+  return LaunchClusters(gemm_i8_pair_kernel<OUT, GELU>, 2 * pairs, PairCfg::kThreads, 2, PairCfg::kSmem, c.st, ta, tb, tc, c.C, (long long)c.ldc, c.M, c.N,
                         c.K, c.ep, tma_store);
 }
 
@@ -614,7 +676,11 @@ int LaunchNoDepth(const Call& c) {
 template <int OUT>
 int LaunchForm(const Call& c, const Form& f) {
   if (c.K == 0) return LaunchNoDepth<OUT>(c);
-  if (f.pair) return LaunchPair<OUT>(c);
+  if constexpr (OUT == kOutS32) {
+    if (f.pair) return LaunchPair<OUT, false>(c);
+  } else {
+    if (f.pair) return c.ep.gelu ? LaunchPair<OUT, true>(c) : LaunchPair<OUT, false>(c);
+  }
   if (f.bt == 32) return LaunchTile<32, OUT>(c, f.splits);
   if (f.bt == 64) return LaunchTile<64, OUT>(c, f.splits);
   return LaunchTile<128, OUT>(c, f.splits);
