@@ -52,19 +52,6 @@ __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float add_rn(float x, float r) { return x + r; }
 __device__ __forceinline__ __nv_bfloat16 add_rn(__nv_bfloat16 x, __nv_bfloat16 r) { return __hadd_rn(x, r); }
 __device__ __forceinline__ __half add_rn(__half x, __half r) { return __hadd_rn(x, r); }
-__device__ __forceinline__ void add_rn2(float* x, const float* r) {
-  x[0] += r[0];
-  x[1] += r[1];
-}
-template <typename T2, typename T>
-__device__ __forceinline__ void add_rn2_16(T* x, const T* r) {
-  const T2 s = __hadd2_rn(T2{x[0], x[1]}, T2{r[0], r[1]});
-  x[0] = s.x;
-  x[1] = s.y;
-}
-__device__ __forceinline__ void add_rn2(__nv_bfloat16* x, const __nv_bfloat16* r) { add_rn2_16<__nv_bfloat162>(x, r); }
-__device__ __forceinline__ void add_rn2(__half* x, const __half* r) { add_rn2_16<__half2>(x, r); }
-
 // Two f32 operations in one instruction.
 struct F2 {
   float x, y;
@@ -93,32 +80,86 @@ __device__ __forceinline__ float max_abs(float m, float a) {
   return d;
 }
 
-// VEC consecutive elements: one 4-, 8- or 16-byte access (two of 16 for eight f32).
-template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC > 16 ? 16 : sizeof(T) * VEC) Pack {
-  T v[VEC];
+// Two elements of a row in registers: one word for a 16-bit type, two for f32.  (Kept as words: arrays of 16-bit
+// values cost the compiler several byte permutes an element.)
+template <typename T>
+constexpr int kPairWords = (int)sizeof(T) / 2;
+template <typename T>
+struct Pair {
+  uint32_t w[kPairWords<T>];
 };
-// Elements at .. at + VEC - 1 of a row of `cols`, those past its end as `none`.
-template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> load_pack(const T* p, int at, int cols, T none) {
-  Pack<T, VEC> k;
-  if (VEC == 1 || at + VEC <= cols) {
-    if (at < cols) k = *reinterpret_cast<const Pack<T, VEC>*>(p + at);
-    else k.v[0] = none;
-  } else {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) k.v[e] = at + e < cols ? p[at + e] : none;
-  }
-  return k;
+__device__ __forceinline__ F2 unpack(Pair<float> p) { return {__uint_as_float(p.w[0]), __uint_as_float(p.w[1])}; }
+__device__ __forceinline__ F2 unpack(Pair<__nv_bfloat16> p) {
+  return {__uint_as_float(p.w[0] << 16), __uint_as_float(p.w[0] & 0xffff0000u)};
 }
-template <typename T, int VEC>
-__device__ __forceinline__ void store_pack(T* p, int at, int cols, const Pack<T, VEC>& k) {
-  if (at + VEC <= cols) {
-    *reinterpret_cast<Pack<T, VEC>*>(p + at) = k;
+__device__ __forceinline__ F2 unpack(Pair<__half> p) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p.w[0]));
+  return {f.x, f.y};
+}
+__device__ __forceinline__ Pair<float> add_rn2(Pair<float> x, Pair<float> r) {
+  const F2 s = add2(unpack(x), unpack(r));
+  return {{__float_as_uint(s.x), __float_as_uint(s.y)}};
+}
+__device__ __forceinline__ Pair<__nv_bfloat16> add_rn2(Pair<__nv_bfloat16> x, Pair<__nv_bfloat16> r) {
+  Pair<__nv_bfloat16> s;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(s.w[0]) : "r"(x.w[0]), "r"(r.w[0]));
+  return s;
+}
+__device__ __forceinline__ Pair<__half> add_rn2(Pair<__half> x, Pair<__half> r) {
+  Pair<__half> s;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(s.w[0]) : "r"(x.w[0]), "r"(r.w[0]));
+  return s;
+}
+
+// The element at j, as bits; 0 past the row's end.
+template <typename T>
+__device__ __forceinline__ uint32_t element_bits(const T* p, int j, int cols) {
+  if (j >= cols) return 0u;
+  if constexpr (sizeof(T) == 4) return *reinterpret_cast<const uint32_t*>(p + j);
+  else return *reinterpret_cast<const uint16_t*>(p + j);
+}
+template <typename T>
+__device__ __forceinline__ Pair<T> make_pair(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(T) == 4) return {{a, b}};
+  else return {{a | b << 16}};
+}
+// Eight elements at j, j + stride, ...: stride 1 is one 16-byte access (two for f32).
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int j, int stride, int cols, Pair<T> (&v)[4]) {
+  if (stride == 1 && j + 8 <= cols) {
+    uint4 u[sizeof(T) / 2];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(p + j)[i];
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < kPairWords<T>; ++k) v[i].w[k] = w[i * kPairWords<T> + k];
   } else {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (at + e < cols) p[at + e] = k.v[e];
+    for (int i = 0; i < 4; ++i)
+      v[i] = make_pair<T>(element_bits(p, j + 2 * i * stride, cols), element_bits(p, j + (2 * i + 1) * stride, cols));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int j, int stride, int cols, const Pair<T> (&v)[4]) {
+  uint32_t w[4 * kPairWords<T>];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int k = 0; k < kPairWords<T>; ++k) w[i * kPairWords<T> + k] = v[i].w[k];
+  if (stride == 1 && j + 8 <= cols) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+      reinterpret_cast<uint4*>(p + j)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int at = j + e * stride;
+      if (at >= cols) continue;
+      if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[at] = w[e];
+      else reinterpret_cast<uint16_t*>(p)[at] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+    }
   }
 }
 
@@ -209,66 +250,59 @@ __device__ __forceinline__ RowScale row_scale(uint32_t mx, float rstd) {
 // 1 / sqrt(ss / n + eps), where ss may be the sum of squares of values scaled by 2^-96.
 __device__ __forceinline__ float inv_rms(float ss, int n, float eps) { return 1.0f / sqrtf(ss / (float)n + eps); }
 
-// One row per warp (!BLOCK) or per block; each thread keeps NV vectors of VEC elements in registers.  All
-// loads of a row are issued before the first is used.
-template <typename T, typename W, bool NORM, int VEC, int NV, bool BLOCK, int MAXT>
+// One row per warp (!BLOCK) or per block; each thread keeps NG groups of eight values in registers: eight
+// neighbours (WIDE), or eight a row of threads apart, where addresses allow no wide access.  All loads of a row
+// are issued before the first is used.
+template <typename T, typename W, bool NORM, bool WIDE, int NG, bool BLOCK, int MAXT>
 __global__ void __launch_bounds__(MAXT) quant_rows_kernel(const RowArgs a) {
   const int tid = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & 31);
-  const int step = BLOCK ? (int)blockDim.x : 32;
+  const int step = BLOCK ? (int)blockDim.x : 32, stride = WIDE ? 1 : step;
   const long long row = BLOCK ? (long long)blockIdx.x : (long long)blockIdx.x * (MAXT / 32) + (threadIdx.x >> 5);
   if (row >= a.rows) return;                     // whole warps (whole blocks) only
   const T* x = (const T*)a.x + row * a.ldx;
   const T* r = NORM && a.r ? (const T*)a.r + row * a.ldr : nullptr;
   T* h = NORM && a.h ? (T*)a.h + row * a.ldh : nullptr;
   const W* w = (const W*)a.w;
-  const T zero = T(0.f);
-  const W wzero = W(0.f);
-  Pack<T, VEC> xv[NV], rv[NORM ? NV : 1];
-  Pack<W, VEC> wv[NORM ? NV : 1];
+  auto first = [&](int g) { return WIDE ? (g * step + tid) * 8 : 8 * g * step + tid; };   // of group g
+  Pair<T> xv[NG][4], rv[NORM ? NG : 1][4];
+  Pair<W> wv[NORM ? NG : 1][4];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) xv[i] = load_pack<T, VEC>(x, (i * step + tid) * VEC, a.cols, zero);
+  for (int g = 0; g < NG; ++g) load8(x, first(g), stride, a.cols, xv[g]);
   if constexpr (NORM) {
     if (r) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) rv[i] = load_pack<T, VEC>(r, (i * step + tid) * VEC, a.cols, zero);
+      for (int g = 0; g < NG; ++g) load8(r, first(g), stride, a.cols, rv[g]);
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) wv[i] = load_pack<W, VEC>(w, (i * step + tid) * VEC, a.cols, wzero);
+    for (int g = 0; g < NG; ++g) load8(w, first(g), stride, a.cols, wv[g]);
     if (r) {
       // h is the sum as it is stored; the norm reads it so, whether or not it is written out
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if constexpr (VEC == 1) {
-          xv[i].v[0] = add_rn(xv[i].v[0], rv[i].v[0]);
-        } else {
+      for (int g = 0; g < NG; ++g) {
 #pragma unroll
-          for (int e = 0; e < VEC; e += 2) add_rn2(&xv[i].v[e], &rv[i].v[e]);
-        }
-        if (h) store_pack<T, VEC>(h, (i * step + tid) * VEC, a.cols, xv[i]);
+        for (int p = 0; p < 4; ++p) xv[g][p] = add_rn2(xv[g][p], rv[g][p]);
+        if (h) store8(h, first(g), stride, a.cols, xv[g]);
       }
     }
   }
-  // The thread's values in pairs, numbered through its vectors.  h stays in its own type and t = h w is formed
-  // anew when it is rounded: fewer registers than t itself.
-  auto h2 = [&](int p) { return F2{to_f32(xv[2 * p / VEC].v[2 * p % VEC]), to_f32(xv[(2 * p + 1) / VEC].v[(2 * p + 1) % VEC])}; };
-  auto t2 = [&](int p) {
-    if constexpr (NORM)
-      return mul2(h2(p), F2{to_f32(wv[2 * p / VEC].v[2 * p % VEC]), to_f32(wv[(2 * p + 1) / VEC].v[(2 * p + 1) % VEC])});
-    else
-      return h2(p);
+  // h stays in its own type and t = h w is formed anew when it is rounded: fewer registers than t itself
+  auto t_of = [&](int g, int p) {
+    if constexpr (NORM) return mul2(unpack(xv[g][p]), unpack(wv[g][p]));
+    else return unpack(xv[g][p]);
   };
-  constexpr int kPairs = NV * VEC / 2;
   F2 ss2 = {0.f, 0.f};
   float mx = 0.f;
 #pragma unroll
-  for (int p = 0; p < kPairs; ++p) {
-    if constexpr (NORM) {
-      const F2 v = h2(p);
-      ss2 = fma2(v, v, ss2);
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      if constexpr (NORM) {
+        const F2 v = unpack(xv[g][p]);
+        ss2 = fma2(v, v, ss2);
+      }
+      const F2 t = t_of(g, p);
+      mx = max_abs(max_abs(mx, t.x), t.y);
     }
-    const F2 t = t2(p);
-    mx = max_abs(max_abs(mx, t.x), t.y);
-  }
   float ss = ss2.x + ss2.y;
   uint32_t top = abs_bits(mx);
   reduce_row<BLOCK, NORM>(ss, top);
@@ -278,10 +312,12 @@ __global__ void __launch_bounds__(MAXT) quant_rows_kernel(const RowArgs a) {
     if (abs_bits(ss) >= kInfBits && top < kInfBits) {  // finite values whose squares overflow: of h * 2^-96
       float s2 = 0.f;
 #pragma unroll
-      for (int p = 0; p < kPairs; ++p) {
-        const F2 v = mul2(h2(p), {kDown, kDown});
-        s2 = fmaf(v.x, v.x, fmaf(v.y, v.y, s2));
-      }
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const F2 v = mul2(unpack(xv[g][p]), {kDown, kDown});
+          s2 = fmaf(v.x, v.x, fmaf(v.y, v.y, s2));
+        }
       uint32_t none = 0;
       reduce_row<BLOCK, true>(s2, none);
       rstd = inv_rms(s2, a.cols, 0.f) * kDown;
@@ -291,21 +327,19 @@ __global__ void __launch_bounds__(MAXT) quant_rows_kernel(const RowArgs a) {
   if (tid == 0) a.scale[row] = s.scale;
   int8_t* q = a.q + row * a.ldq;
 #pragma unroll
-  for (int g = 0; g < kPairs / 4; ++g) {         // eight values at a time: a vector, or eight of one element
-    const int at = (VEC == 1 ? 8 * g * step + tid : (g * step + tid) * 8);
+  for (int g = 0; g < NG; ++g) {
+    const int at = first(g);
     if (at >= a.cols) continue;
-    const F2 t[4] = {t2(4 * g), t2(4 * g + 1), t2(4 * g + 2), t2(4 * g + 3)};
+    const F2 t[4] = {t_of(g, 0), t_of(g, 1), t_of(g, 2), t_of(g, 3)};
     const uint2 k = s.live ? round8(t, s.inv, s.m) : make_uint2(0u, 0u);
-    if constexpr (VEC == 8) {
-      if (at + 8 <= a.cols) {
-        *reinterpret_cast<uint2*>(q + at) = k;
-        continue;
-      }
-    }
+    if (WIDE && at + 8 <= a.cols) {
+      *reinterpret_cast<uint2*>(q + at) = k;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int j = at + (VEC == 1 ? e * step : e);
-      if (j < a.cols) q[j] = (int8_t)((e < 4 ? k.x : k.y) >> (8 * (e & 3)));
+      for (int e = 0; e < 8; ++e) {
+        const int j = at + e * stride;
+        if (j < a.cols) q[j] = (int8_t)((e < 4 ? k.x : k.y) >> (8 * (e & 3)));
+      }
     }
   }
 }
@@ -361,15 +395,15 @@ __global__ void __launch_bounds__(kMaxThreads) quant_long_rows_kernel(const RowA
 }
 
 // The launch of a row: `threads` of them, 32 for a warp.
-template <typename T, typename W, bool NORM, int VEC, int NV>
-void LaunchBlock(const RowArgs& a, int vecs, cudaStream_t st) {
-  const int threads = ((vecs + NV - 1) / NV + 31) / 32 * 32;
-  if (threads <= 256) quant_rows_kernel<T, W, NORM, VEC, NV, true, 256><<<a.rows, threads, 0, st>>>(a);
-  else quant_rows_kernel<T, W, NORM, VEC, NV, true, kMaxThreads><<<a.rows, threads, 0, st>>>(a);
+template <typename T, typename W, bool NORM, bool WIDE, int NG>
+void LaunchBlock(const RowArgs& a, int groups, cudaStream_t st) {
+  const int threads = ((groups + NG - 1) / NG + 31) / 32 * 32;
+  if (threads <= 256) quant_rows_kernel<T, W, NORM, WIDE, NG, true, 256><<<a.rows, threads, 0, st>>>(a);
+  else quant_rows_kernel<T, W, NORM, WIDE, NG, true, kMaxThreads><<<a.rows, threads, 0, st>>>(a);
 }
-template <typename T, typename W, bool NORM, int VEC, int NV>
+template <typename T, typename W, bool NORM, bool WIDE, int NG>
 void LaunchWarp(const RowArgs& a, cudaStream_t st) {
-  quant_rows_kernel<T, W, NORM, VEC, NV, false, 128><<<(a.rows + 3) / 4, 128, 0, st>>>(a);
+  quant_rows_kernel<T, W, NORM, WIDE, NG, false, 128><<<(a.rows + 3) / 4, 128, 0, st>>>(a);
 }
 
 template <typename T, typename W, bool NORM>
@@ -378,22 +412,22 @@ void LaunchTW(const RowArgs& a, cudaStream_t st) {
   const bool wide = at16(a.x, a.ldx) && (uintptr_t)a.q % 8 == 0 && a.ldq % 8 == 0 &&
                     (!NORM || ((!a.r || at16(a.r, a.ldr)) && (!a.h || at16(a.h, a.ldh)) && (uintptr_t)a.w % 16 == 0));
   const bool many = a.rows >= 148 * 8;
+  const int groups = (a.cols + 7) / 8;
   if (wide) {
-    const int vecs = (a.cols + 7) / 8;
-    if (vecs <= 32 || (many && vecs <= 128)) {
-      if (vecs <= 32) return LaunchWarp<T, W, NORM, 8, 1>(a, st);
-      if (vecs <= 64) return LaunchWarp<T, W, NORM, 8, 2>(a, st);
-      if (vecs <= 96) return LaunchWarp<T, W, NORM, 8, 3>(a, st);
-      return LaunchWarp<T, W, NORM, 8, 4>(a, st);
+    if (groups <= 32 || (many && groups <= 128)) {
+      if (groups <= 32) return LaunchWarp<T, W, NORM, true, 1>(a, st);
+      if (groups <= 64) return LaunchWarp<T, W, NORM, true, 2>(a, st);
+      if (groups <= 96) return LaunchWarp<T, W, NORM, true, 3>(a, st);
+      return LaunchWarp<T, W, NORM, true, 4>(a, st);
     }
-    if (vecs <= 256 || (!many && vecs <= kMaxThreads)) return LaunchBlock<T, W, NORM, 8, 1>(a, vecs, st);
-    if (vecs <= 512) return LaunchBlock<T, W, NORM, 8, 2>(a, vecs, st);
-    if (vecs <= 2 * kMaxThreads && (sizeof(T) == 4 || sizeof(W) == 4)) return LaunchBlock<T, W, NORM, 8, 2>(a, vecs, st);
-    if (vecs <= 4 * kMaxThreads) return LaunchBlock<T, W, NORM, 8, 4>(a, vecs, st);
+    if (groups <= 256 || (!many && groups <= kMaxThreads)) return LaunchBlock<T, W, NORM, true, 1>(a, groups, st);
+    if (groups <= 512) return LaunchBlock<T, W, NORM, true, 2>(a, groups, st);
+    if (groups <= 2 * kMaxThreads && (sizeof(T) == 4 || sizeof(W) == 4)) return LaunchBlock<T, W, NORM, true, 2>(a, groups, st);
+    if (groups <= 4 * kMaxThreads) return LaunchBlock<T, W, NORM, true, 4>(a, groups, st);
   } else {
-    if (a.cols <= 256) return LaunchWarp<T, W, NORM, 1, 8>(a, st);
-    if (a.cols <= 8 * kMaxThreads) return LaunchBlock<T, W, NORM, 1, 8>(a, a.cols, st);
-    if (a.cols <= 32 * kMaxThreads) return LaunchBlock<T, W, NORM, 1, 32>(a, a.cols, st);
+    if (groups <= 32) return LaunchWarp<T, W, NORM, false, 1>(a, st);
+    if (groups <= kMaxThreads) return LaunchBlock<T, W, NORM, false, 1>(a, groups, st);
+    if (groups <= 4 * kMaxThreads) return LaunchBlock<T, W, NORM, false, 4>(a, groups, st);
   }
   quant_long_rows_kernel<T, W, NORM><<<a.rows, kMaxThreads, 0, st>>>(a);
 }
