@@ -6,9 +6,9 @@
 // The norm's factor is the same for the whole row, so it cancels in q and enters the scale alone: a row
 // needs one reduction of the pair (sum h^2, max |t|), after which every value is rounded from registers.
 //
-// q is the exact quotient's rounding, not that of f32 arithmetic: t * (127 / m) is off by less than
-// 127 * 2^-23 = 1.6e-5, so a value further than kBorder = 2^-15 from a border between two integers is
-// rounded right in f32, and the few others (6e-5 of them) are divided in 64 bits, where the quotient of
+// q is the exact quotient's rounding, not that of f32 arithmetic: t * (127 / m) is off by less than 2^-14.9, so
+// a value further than 2^-14 from a border between two integers is rounded right in f32, and the few others
+// (1.2e-4 of them) are divided in 64 bits, where the quotient of
 // two f32 values cannot cross or miss a border.  The result then depends on no order of operations.
 //
 // The maximum keeps a NaN, and across threads it is taken on the bit patterns of |t| as integers, which order
@@ -26,7 +26,7 @@ namespace b200k {
 namespace {
 
 constexpr uint32_t kInfBits = 0x7f800000u;
-constexpr float kBorder = 0.5f - 1.0f / 32768.0f;
+constexpr float kBorder = 0.5f - 1.0f / 16384.0f;
 constexpr float kRoundMagic = 12582912.0f;     // 1.5 * 2^23: adding it rounds |v| < 2^22 to an integer
 constexpr float kDown = 1.262177448353619e-29f;    // 2^-96
 constexpr int kMaxThreads = 1024;
@@ -73,10 +73,10 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
   return floats(d);
 }
-// The larger of m and |a|; NaN if either is.
-__device__ __forceinline__ float max_abs(float m, float a) {
+// The largest of m, |a.x| and |a.y|; NaN if one of them is.
+__device__ __forceinline__ float max_abs(float m, F2 a) {
   float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(m), "f"(fabsf(a)));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(fabsf(a.x)), "f"(fabsf(a.y)));
   return d;
 }
 
@@ -111,56 +111,114 @@ __device__ __forceinline__ Pair<__half> add_rn2(Pair<__half> x, Pair<__half> r) 
   return s;
 }
 
-// The element at j, as bits; 0 past the row's end.
-template <typename T>
-__device__ __forceinline__ uint32_t element_bits(const T* p, int j, int cols) {
-  if (j >= cols) return 0u;
-  if constexpr (sizeof(T) == 4) return *reinterpret_cast<const uint32_t*>(p + j);
-  else return *reinterpret_cast<const uint16_t*>(p + j);
-}
-template <typename T>
-__device__ __forceinline__ Pair<T> make_pair(uint32_t a, uint32_t b) {
-  if constexpr (sizeof(T) == 4) return {{a, b}};
-  else return {{a | b << 16}};
-}
-// Eight elements at j, j + stride, ...: stride 1 is one 16-byte access (two for f32).
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int j, int stride, int cols, Pair<T> (&v)[4]) {
-  if (stride == 1 && j + 8 <= cols) {
-    uint4 u[sizeof(T) / 2];
+// Drops the first `bytes` of NW + EX words; the NW that follow remain.
+template <int NW, int EX>
+__device__ __forceinline__ void drop_bytes(uint32_t (&x)[NW + EX], int bytes) {
+  if constexpr (EX == 4) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(p + j)[i];
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(u);
+    for (int i = 0; i < NW + 2; ++i) x[i] = bytes & 8 ? x[i + 2] : x[i];
+  }
+#pragma unroll
+  for (int i = 0; i < NW + 1; ++i) x[i] = bytes & 4 ? x[i + 1] : x[i];
+#pragma unroll
+  for (int i = 0; i < NW; ++i) x[i] = __funnelshift_r(x[i], x[i + 1], 8 * (bytes & 3));
+}
+
+// The 16-byte lines that hold the eight neighbours p[j ..] of a row.  ALIGNED: they are those lines.  Else the
+// lines are read whole (one that holds a byte of the row lies in the row's allocation) and shifted afterwards: two
+// wide loads and some twenty integer operations in the place of eight narrow loads.  Nothing here reads what was
+// loaded, so that the loads of all groups and arrays are in flight together.
+template <typename T, bool ALIGNED>
+struct Lines {
+  static constexpr int kWords = 4 * kPairWords<T>, kLines = kWords / 4 + (ALIGNED ? 0 : 1);
+  uint4 u[kLines];
+  __device__ __forceinline__ void load(const T* p, int j, int cols) {
+    const char* at = reinterpret_cast<const char*>(p + j);
+    const char* end = reinterpret_cast<const char*>(p + cols);
+    const char* line = ALIGNED ? at : at - ((uintptr_t)at & 15);
+#pragma unroll
+    for (int i = 0; i < kLines; ++i) {
+      u[i] = make_uint4(0u, 0u, 0u, 0u);
+      if ((unsigned)j < (unsigned)cols && line + 16 * i < end) u[i] = *reinterpret_cast<const uint4*>(line + 16 * i);
+    }
+  }
+  // The eight elements; 0 past the row's end.
+  __device__ __forceinline__ void take(const T* p, int j, int cols, Pair<T> (&v)[4]) const {
+    uint32_t x[kWords + 4];
+#pragma unroll
+    for (int i = 0; i < kLines; ++i) {
+      x[4 * i] = u[i].x;
+      x[4 * i + 1] = u[i].y;
+      x[4 * i + 2] = u[i].z;
+      x[4 * i + 3] = u[i].w;
+    }
+    if constexpr (!ALIGNED) drop_bytes<kWords, 4>(x, (int)((uintptr_t)(p + j) & 15));
+    if (j + 8 > cols) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {         // the word's elements past the end
+        const int e = j + i * 4 / (int)sizeof(T);
+        if (e >= cols) x[i] = 0;
+        else if (sizeof(T) == 2 && e + 1 >= cols) x[i] &= 0xffffu;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int k = 0; k < kPairWords<T>; ++k) v[i].w[k] = w[i * kPairWords<T> + k];
+      for (int k = 0; k < kPairWords<T>; ++k) v[i].w[k] = x[i * kPairWords<T> + k];
+  }
+};
+
+// Eight neighbours to p[j ..], nothing past the row's end.  Else than ALIGNED, a lane writes the whole lines that
+// begin with the last bytes of the group before it, which the lane before it holds; those at the row's ends are
+// written element by element.  Every lane of the warp calls this; a lane that is `mute` only hands on its group.
+template <typename E, int NW, bool ALIGNED>
+__device__ __forceinline__ void store8(E* p, int j, int cols, const uint32_t (&w)[NW], bool mute) {
+  constexpr int EX = NW < 4 ? NW : 4, kLine = 4 * EX;
+  auto element = [&](const uint32_t* x, int e) {
+    if constexpr (sizeof(E) == 4) return x[e];
+    else if constexpr (sizeof(E) == 2) return (x[e / 2] >> (16 * (e & 1))) & 0xffffu;
+    else return (x[e / 4] >> (8 * (e & 3))) & 0xffu;
+  };
+  auto put = [&](int at, uint32_t bits) {
+    if constexpr (sizeof(E) == 4) reinterpret_cast<uint32_t*>(p)[at] = bits;
+    else if constexpr (sizeof(E) == 2) reinterpret_cast<uint16_t*>(p)[at] = (uint16_t)bits;
+    else reinterpret_cast<uint8_t*>(p)[at] = (uint8_t)bits;
+  };
+  auto whole = [&](int at, const uint32_t* x) {
+#pragma unroll
+    for (int i = 0; i < NW; i += EX) {
+      if constexpr (EX == 4) reinterpret_cast<uint4*>(p + at)[i / 4] = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+      else *reinterpret_cast<uint2*>(p + at) = make_uint2(x[0], x[1]);
+    }
+  };
+  const int off = ALIGNED ? 0 : (int)((uintptr_t)(p + j) & (kLine - 1));   // the same for all lanes of a row
+  uint32_t x[NW + EX];
+#pragma unroll
+  for (int i = 0; i < EX; ++i) x[i] = ALIGNED ? 0u : __shfl_up_sync(0xffffffffu, w[NW - EX + i], 1);
+#pragma unroll
+  for (int i = 0; i < NW; ++i) x[EX + i] = w[i];
+  const int from = j - off / (int)sizeof(E);
+  if (ALIGNED || off == 0) {
+#pragma unroll
+    for (int i = 0; i < NW; ++i) x[i] = w[i];
+  } else {
+    drop_bytes<NW, EX>(x, kLine - off);
+  }
+  if (mute) return;
+  if (from >= 0 && from + 8 <= cols) {
+    whole(from, x);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = make_pair<T>(element_bits(p, j + 2 * i * stride, cols), element_bits(p, j + (2 * i + 1) * stride, cols));
+    for (int e = 0; e < 8; ++e)
+      if (from + e >= 0 && from + e < cols) put(from + e, element(x, e));
   }
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, int j, int stride, int cols, const Pair<T> (&v)[4]) {
-  uint32_t w[4 * kPairWords<T>];
+__device__ __forceinline__ void words_of(const Pair<T> (&v)[4], uint32_t (&w)[4 * kPairWords<T>]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int k = 0; k < kPairWords<T>; ++k) w[i * kPairWords<T> + k] = v[i].w[k];
-  if (stride == 1 && j + 8 <= cols) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-      reinterpret_cast<uint4*>(p + j)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int at = j + e * stride;
-      if (at >= cols) continue;
-      if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[at] = w[e];
-      else reinterpret_cast<uint16_t*>(p)[at] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
-    }
-  }
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -168,16 +226,16 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v
 // The few values next to a border, out of line: 127 t / m in 64 bits.
 __device__ __noinline__ uint32_t round_exact(float t, float m) { return (uint32_t)__double2int_rn(127.0 * (double)t / (double)m); }
 
+// round_half_even(127 t / m), of which the low byte counts; inv as row_round gives it.
 __device__ __forceinline__ uint32_t round_i8(float t, float inv, float m) {
   const float v = t * inv;
   const float s = v + kRoundMagic;
-  // also taken where inv overflowed (m below 127 / FLT_MAX) and v is no number
   if (!(fabsf(v - (s - kRoundMagic)) < kBorder)) return round_exact(t, m);
   return __float_as_uint(s);
 }
 
-// round_half_even(127 t_i / m) of eight values, packed into 8 bytes; inv = 127 / m in f32, off where it is not
-// finite (m below 127 / FLT_MAX).  One branch for the eight: 1.5 % of warps have a value next to a border.
+// round_half_even(127 t_i / m) of eight values, packed into 8 bytes; inv as row_round gives it.  One
+// branch for the eight: 3 % of warps have a value next to a border.
 __device__ __noinline__ uint2 round8_exact(F2 a, F2 b, F2 c, F2 d, float m) {
   const float t[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
   uint32_t q[2] = {0, 0};
@@ -199,22 +257,24 @@ __device__ __forceinline__ uint2 round8(const F2 (&t)[4], float inv, float m) {
     s[i] = add2(v, {kRoundMagic, kRoundMagic});
     const F2 k = add2(s[i], {-kRoundMagic, -kRoundMagic});
     const F2 d = fma2(k, {-1.f, -1.f}, v);
-    far = max_abs(max_abs(far, d.x), d.y);       // NaN where inv is not finite
+    far = max_abs(far, d);                       // NaN where inv is
   }
   if (!(far < kBorder)) return round8_exact(t[0], t[1], t[2], t[3], m);
   return make_uint2(low_bytes(s[0].x, s[0].y, s[1].x, s[1].y), low_bytes(s[2].x, s[2].y, s[3].x, s[3].y));
 }
 
-// Sum and maximum over the threads of one row: the warp, or (BLOCK) the whole block.
-template <bool BLOCK, bool SUM>
+// Sum and maximum over the threads of one row: LANES of a warp, or (LANES 0) the whole block.
+template <int LANES, bool SUM, int PLACE>
 __device__ __forceinline__ void reduce_row(float& ss, uint32_t& mx) {
-  if (SUM) {
+  constexpr int kIn = LANES ? LANES : 32;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  for (int o = kIn / 2; o; o >>= 1) {
+    if (SUM) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (kIn < 32) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
-  mx = __reduce_max_sync(0xffffffffu, mx);
-  if constexpr (BLOCK) {
-    __shared__ float s_ss[32];
+  if (kIn == 32) mx = __reduce_max_sync(0xffffffffu, mx);
+  if constexpr (LANES == 0) {
+    __shared__ float s_ss[32];                   // one set for each place that reduces
     __shared__ uint32_t s_mx[32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     if (lane == 0) {
@@ -224,7 +284,6 @@ __device__ __forceinline__ void reduce_row(float& ss, uint32_t& mx) {
     __syncthreads();
     ss = lane < warps ? s_ss[lane] : 0.f;
     mx = lane < warps ? s_mx[lane] : 0u;
-    __syncthreads();                             // the slots may be written again
     if (SUM) {
 #pragma unroll
       for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -233,83 +292,126 @@ __device__ __forceinline__ void reduce_row(float& ss, uint32_t& mx) {
   }
 }
 
-// What a row's reduction says: 127 / m (0 for a row of zeros or of values that are no numbers), m, and
-// the scale.
-struct RowScale {
-  float inv, m, scale;
-  bool live;
+// How a row whose largest |t| has the bits `mx` is rounded: 127 / m, or NaN for an m too small or too large for
+// that to be exact enough (its values are then divided one by one).  The reciprocal is off by 2^-23, the products
+// with 127 and with t by 2^-24 each: the quotient of at most 127 by less than 2^-14.9.
+struct RowRound {
+  float inv, m;
+  bool live;                                     // not all zeros, and all numbers
 };
-__device__ __forceinline__ RowScale row_scale(uint32_t mx, float rstd) {
-  RowScale s;
+__device__ __forceinline__ RowRound row_round(uint32_t mx) {
+  RowRound s;
   s.m = __uint_as_float(mx);
   s.live = mx != 0 && mx < kInfBits;
-  s.inv = s.live ? 127.0f / s.m : 0.f;
-  s.scale = mx >= kInfBits ? __uint_as_float(0x7fc00000u) : s.m / 127.0f * rstd;
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s.m));
+  s.inv = s.m > 1e-36f && s.m < 1e37f ? 127.0f * r : __uint_as_float(0x7fc00000u);
   return s;
 }
-// 1 / sqrt(ss / n + eps), where ss may be the sum of squares of values scaled by 2^-96.
-__device__ __forceinline__ float inv_rms(float ss, int n, float eps) { return 1.0f / sqrtf(ss / (float)n + eps); }
+// m / 127 [* 1 / sqrt(mean(h^2) + eps)]; ss is the sum of squares of down * h.
+template <bool NORM>
+__device__ __forceinline__ float row_scale(uint32_t mx, float ss, float down, int n, float eps) {
+  if (mx >= kInfBits) return __uint_as_float(0x7fc00000u);
+  const float s = __uint_as_float(mx) / 127.0f;
+  if (!NORM) return s;
+  return s * (1.0f / sqrtf(ss / (float)n + (down == 1.f ? eps : 0.f)) * down);   // (eps vanishes beside such squares)
+}
 
-// One row per warp (!BLOCK) or per block; each thread keeps NG groups of eight values in registers: eight
-// neighbours (WIDE), or eight a row of threads apart, where addresses allow no wide access.  All loads of a row
-// are issued before the first is used.
-template <typename T, typename W, bool NORM, bool WIDE, int NG, bool BLOCK, int MAXT>
+// One row per LANES lanes of a warp, or (LANES 0) per block; each thread keeps NG groups of eight neighbours in
+// registers.  All loads of a row are issued before the first is used.
+//
+// Rows that are not ALIGNED and take more than one warp's groups are dealt out to 31 lanes of a warp, and lane 0
+// holds the group before them once more: the lines that two groups share are then written by one lane wherever
+// they lie, and only a row's two ends are written element by element.
+template <typename T, typename W, bool NORM, bool ALIGNED, int NG, int LANES, int MAXT>
 __global__ void __launch_bounds__(MAXT) quant_rows_kernel(const RowArgs a) {
-  const int tid = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & 31);
-  const int step = BLOCK ? (int)blockDim.x : 32, stride = WIDE ? 1 : step;
-  const long long row = BLOCK ? (long long)blockIdx.x : (long long)blockIdx.x * (MAXT / 32) + (threadIdx.x >> 5);
-  if (row >= a.rows) return;                     // whole warps (whole blocks) only
+  constexpr int kLanes = LANES ? LANES : 32;
+  const int tid = LANES ? (int)(threadIdx.x & (kLanes - 1)) : (int)threadIdx.x;
+  const int step = LANES ? kLanes : (int)blockDim.x;
+  const long long mine = LANES ? ((long long)blockIdx.x * MAXT + threadIdx.x) / kLanes : (long long)blockIdx.x;
+  // lanes past the last row go with their warp: they hold zeros and write nothing
+  const long long row = min(mine, (long long)a.rows - 1);
+  const int cols = mine < a.rows ? a.cols : 0;
   const T* x = (const T*)a.x + row * a.ldx;
   const T* r = NORM && a.r ? (const T*)a.r + row * a.ldr : nullptr;
   T* h = NORM && a.h ? (T*)a.h + row * a.ldh : nullptr;
   const W* w = (const W*)a.w;
-  auto first = [&](int g) { return WIDE ? (g * step + tid) * 8 : 8 * g * step + tid; };   // of group g
-  Pair<T> xv[NG][4], rv[NORM ? NG : 1][4];
+  constexpr bool kTwice = !ALIGNED && (LANES == 0 || NG > 1);
+  const bool again = kTwice && (threadIdx.x & 31) == 0;         // holds a group of the lane before it
+  // the thread's g-th group begins here (before 0 or past the end: none)
+  Pair<T> xv[NG][4];
   Pair<W> wv[NORM ? NG : 1][4];
+  auto first = [&](int g) {
+    if constexpr (!kTwice) return (g * step + tid) * 8;
+    else return ((g * (step >> 5) + (tid >> 5)) * 31 + (tid & 31) - 1) * 8;
+  };
+  auto write_h = [&](int g) {
+    uint32_t words[4 * kPairWords<T>];
+    words_of(xv[g], words);
+    store8<T, 4 * kPairWords<T>, ALIGNED>(h, first(g), cols, words, again);
+  };
+  Lines<T, ALIGNED> xl[NG], rl[NORM ? NG : 1];
+  Lines<W, ALIGNED> wl[NORM ? NG : 1];
 #pragma unroll
-  for (int g = 0; g < NG; ++g) load8(x, first(g), stride, a.cols, xv[g]);
+  for (int g = 0; g < NG; ++g) xl[g].load(x, first(g), cols);
   if constexpr (NORM) {
-    if (r) {
 #pragma unroll
-      for (int g = 0; g < NG; ++g) load8(r, first(g), stride, a.cols, rv[g]);
+    for (int g = 0; g < NG; ++g) {
+      rl[g].load(r, first(g), r ? cols : 0);
+      if (ALIGNED) wl[g].load(w, first(g), cols);
     }
+  }
 #pragma unroll
-    for (int g = 0; g < NG; ++g) load8(w, first(g), stride, a.cols, wv[g]);
+  for (int g = 0; g < NG; ++g) xl[g].take(x, first(g), cols, xv[g]);
+  if constexpr (NORM) {
     if (r) {
       // h is the sum as it is stored; the norm reads it so, whether or not it is written out
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
+        Pair<T> rv[4];
+        rl[g].take(r, first(g), cols, rv);
 #pragma unroll
-        for (int p = 0; p < 4; ++p) xv[g][p] = add_rn2(xv[g][p], rv[g][p]);
-        if (h) store8(h, first(g), stride, a.cols, xv[g]);
+        for (int p = 0; p < 4; ++p) xv[g][p] = add_rn2(xv[g][p], rv[p]);
+        if (ALIGNED && h) write_h(g);
       }
     }
+    // (lines that have to be shifted take twice the registers: the weights', which every row reads, come last)
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      if (!ALIGNED) wl[g].load(w, first(g), cols);
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) wl[g].take(w, first(g), cols, wv[g]);
   }
-  // h stays in its own type and t = h w is formed anew when it is rounded: fewer registers than t itself
-  auto t_of = [&](int g, int p) {
-    if constexpr (NORM) return mul2(unpack(xv[g][p]), unpack(wv[g][p]));
-    else return unpack(xv[g][p]);
-  };
-  F2 ss2 = {0.f, 0.f};
+  F2 t[NG][4], ss2 = {0.f, 0.f};
   float mx = 0.f;
 #pragma unroll
   for (int g = 0; g < NG; ++g)
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
+      t[g][p] = unpack(xv[g][p]);
       if constexpr (NORM) {
-        const F2 v = unpack(xv[g][p]);
-        ss2 = fma2(v, v, ss2);
+        ss2 = fma2(t[g][p], t[g][p], ss2);
+        t[g][p] = mul2(t[g][p], unpack(wv[g][p]));
       }
-      const F2 t = t_of(g, p);
-      mx = max_abs(max_abs(mx, t.x), t.y);
+      mx = max_abs(mx, t[g][p]);
     }
-  float ss = ss2.x + ss2.y;
+  float ss = again ? 0.f : ss2.x + ss2.y;
   uint32_t top = abs_bits(mx);
-  reduce_row<BLOCK, NORM>(ss, top);
-  float rstd = 1.f;
+  reduce_row<LANES, NORM, 0>(ss, top);
   if constexpr (NORM) {
-    rstd = inv_rms(ss, a.cols, a.eps);
-    if (abs_bits(ss) >= kInfBits && top < kInfBits) {  // finite values whose squares overflow: of h * 2^-96
+    // Lanes write each other's elements here, and h may lie over x or r: after the reduction, which a thread
+    // enters with its loads done.
+    if (!ALIGNED && h) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) write_h(g);
+    }
+  }
+  float down = 1.f;                              // what h was multiplied by for ss
+  if constexpr (NORM) {
+    // finite values whose squares overflow: of h * 2^-96 (the rows of a warp go there together)
+    const bool over = abs_bits(ss) >= kInfBits && top < kInfBits;
+    if (LANES == 0 ? over : __any_sync(0xffffffffu, over)) {
       float s2 = 0.f;
 #pragma unroll
       for (int g = 0; g < NG; ++g)
@@ -318,29 +420,23 @@ __global__ void __launch_bounds__(MAXT) quant_rows_kernel(const RowArgs a) {
           const F2 v = mul2(unpack(xv[g][p]), {kDown, kDown});
           s2 = fmaf(v.x, v.x, fmaf(v.y, v.y, s2));
         }
+      if (again) s2 = 0.f;
       uint32_t none = 0;
-      reduce_row<BLOCK, true>(s2, none);
-      rstd = inv_rms(s2, a.cols, 0.f) * kDown;
+      reduce_row<LANES, true, 1>(s2, none);
+      if (over) {
+        ss = s2;
+        down = kDown;
+      }
     }
   }
-  const RowScale s = row_scale(top, rstd);
-  if (tid == 0) a.scale[row] = s.scale;
+  if (tid == 0 && mine < a.rows) a.scale[row] = row_scale<NORM>(top, ss, down, a.cols, a.eps);
+  const RowRound s = row_round(top);
   int8_t* q = a.q + row * a.ldq;
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    const int at = first(g);
-    if (at >= a.cols) continue;
-    const F2 t[4] = {t_of(g, 0), t_of(g, 1), t_of(g, 2), t_of(g, 3)};
-    const uint2 k = s.live ? round8(t, s.inv, s.m) : make_uint2(0u, 0u);
-    if (WIDE && at + 8 <= a.cols) {
-      *reinterpret_cast<uint2*>(q + at) = k;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = at + e * stride;
-        if (j < a.cols) q[j] = (int8_t)((e < 4 ? k.x : k.y) >> (8 * (e & 3)));
-      }
-    }
+    const uint2 k = s.live ? round8(t[g], s.inv, s.m) : make_uint2(0u, 0u);
+    const uint32_t words[2] = {k.x, k.y};
+    store8<int8_t, 2, ALIGNED>(q, first(g), cols, words, again);
   }
 }
 
@@ -372,72 +468,82 @@ __global__ void __launch_bounds__(kMaxThreads) quant_long_rows_kernel(const RowA
     ss = fmaf(v, v, ss);
     mx = max(mx, abs_bits(t_of(v, j)));
   }
-  reduce_row<true, NORM>(ss, mx);
-  float rstd = 1.f;
+  reduce_row<0, NORM, 0>(ss, mx);
+  float down = 1.f;
   if constexpr (NORM) {
-    rstd = inv_rms(ss, a.cols, a.eps);
     if (abs_bits(ss) >= kInfBits && mx < kInfBits) {
-      float s2 = 0.f;
+      ss = 0.f;
       for (long long j = threadIdx.x; j < a.cols; j += blockDim.x) {
         const float v = value(j, false) * kDown;
-        s2 = fmaf(v, v, s2);
+        ss = fmaf(v, v, ss);
       }
       uint32_t none = 0;
-      reduce_row<true, true>(s2, none);
-      rstd = inv_rms(s2, a.cols, 0.f) * kDown;
+      reduce_row<0, true, 1>(ss, none);
+      down = kDown;
     }
   }
-  const RowScale s = row_scale(mx, rstd);
-  if (threadIdx.x == 0) a.scale[row] = s.scale;
+  if (threadIdx.x == 0) a.scale[row] = row_scale<NORM>(mx, ss, down, a.cols, a.eps);
+  const RowRound s = row_round(mx);
   int8_t* q = a.q + row * a.ldq;
   for (long long j = threadIdx.x; j < a.cols; j += blockDim.x)
     q[j] = (int8_t)(s.live ? round_i8(t_of(value(j, false), j), s.inv, s.m) : 0u);
 }
 
-// The launch of a row: `threads` of them, 32 for a warp.
-template <typename T, typename W, bool NORM, bool WIDE, int NG>
+template <typename T, typename W, bool NORM, bool ALIGNED, int NG>
 void LaunchBlock(const RowArgs& a, int groups, cudaStream_t st) {
-  const int threads = ((groups + NG - 1) / NG + 31) / 32 * 32;
-  if (threads <= 256) quant_rows_kernel<T, W, NORM, WIDE, NG, true, 256><<<a.rows, threads, 0, st>>>(a);
-  else quant_rows_kernel<T, W, NORM, WIDE, NG, true, kMaxThreads><<<a.rows, threads, 0, st>>>(a);
+  // not aligned: 31 groups a warp, and a lane past the last group, which writes the end of its last line
+  const int per = ALIGNED ? 32 * NG : 31 * NG, threads = ((groups + (ALIGNED ? 0 : 1) + per - 1) / per) * 32;
+  if (threads <= 256) quant_rows_kernel<T, W, NORM, ALIGNED, NG, 0, 256><<<a.rows, threads, 0, st>>>(a);
+  else if (threads <= 512) quant_rows_kernel<T, W, NORM, ALIGNED, NG, 0, 512><<<a.rows, threads, 0, st>>>(a);
+  else quant_rows_kernel<T, W, NORM, ALIGNED, NG, 0, kMaxThreads><<<a.rows, threads, 0, st>>>(a);
 }
-template <typename T, typename W, bool NORM, bool WIDE, int NG>
+template <typename T, typename W, bool NORM, bool ALIGNED, int NG, int LANES>
 void LaunchWarp(const RowArgs& a, cudaStream_t st) {
-  quant_rows_kernel<T, W, NORM, WIDE, NG, false, 128><<<(a.rows + 3) / 4, 128, 0, st>>>(a);
+  constexpr int kRows = 128 / LANES;
+  quant_rows_kernel<T, W, NORM, ALIGNED, NG, LANES, 128><<<(unsigned)(((long long)a.rows + kRows - 1) / kRows), 128, 0, st>>>(a);
 }
 
-template <typename T, typename W, bool NORM>
+template <typename T, typename W, bool NORM, bool ALIGNED>
 void LaunchTW(const RowArgs& a, cudaStream_t st) {
-  auto at16 = [](const void* p, long long ld) { return (uintptr_t)p % 16 == 0 && ld * (long long)sizeof(T) % 16 == 0; };
-  const bool wide = at16(a.x, a.ldx) && (uintptr_t)a.q % 8 == 0 && a.ldq % 8 == 0 &&
-                    (!NORM || ((!a.r || at16(a.r, a.ldr)) && (!a.h || at16(a.h, a.ldh)) && (uintptr_t)a.w % 16 == 0));
   const bool many = a.rows >= 148 * 8;
   const int groups = (a.cols + 7) / 8;
-  if (wide) {
-    if (groups <= 32 || (many && groups <= 128)) {
-      if (groups <= 32) return LaunchWarp<T, W, NORM, true, 1>(a, st);
-      if (groups <= 64) return LaunchWarp<T, W, NORM, true, 2>(a, st);
-      if (groups <= 96) return LaunchWarp<T, W, NORM, true, 3>(a, st);
-      return LaunchWarp<T, W, NORM, true, 4>(a, st);
-    }
-    if (groups <= 256 || (!many && groups <= kMaxThreads)) return LaunchBlock<T, W, NORM, true, 1>(a, groups, st);
-    if (groups <= 512) return LaunchBlock<T, W, NORM, true, 2>(a, groups, st);
-    if (groups <= 2 * kMaxThreads && (sizeof(T) == 4 || sizeof(W) == 4)) return LaunchBlock<T, W, NORM, true, 2>(a, groups, st);
+  const int lanes = groups + (ALIGNED ? 0 : 1);  // see LaunchBlock
+  if (lanes <= 8) return LaunchWarp<T, W, NORM, ALIGNED, 1, 8>(a, st);
+  if (lanes <= 16) return LaunchWarp<T, W, NORM, ALIGNED, 1, 16>(a, st);
+  if (lanes <= 32) return LaunchWarp<T, W, NORM, ALIGNED, 1, 32>(a, st);
+  if constexpr (ALIGNED) {
+    // Few rows: as many threads a row as it has groups (latency).  Many: more groups a thread, so that more bytes
+    // are in flight for each reduction; norm rows, with three times the registers, best at two (bf16 16384 x 4096:
+    // 103, 78, 87 us with 1, 2, 4 groups), quantised rows at four (62, 47, 41 us).
+    if (!many && groups <= kMaxThreads) return LaunchBlock<T, W, NORM, true, 1>(a, groups, st);
+    if (groups <= 64) return LaunchWarp<T, W, NORM, true, 2, 32>(a, st);
+    if (groups <= 96) return LaunchWarp<T, W, NORM, true, 3, 32>(a, st);
+    if (!NORM && groups <= 128) return LaunchWarp<T, W, NORM, true, 4, 32>(a, st);
+    if (NORM && groups <= 2 * kMaxThreads) return LaunchBlock<T, W, NORM, true, 2>(a, groups, st);
     if (groups <= 4 * kMaxThreads) return LaunchBlock<T, W, NORM, true, 4>(a, groups, st);
   } else {
-    if (groups <= 32) return LaunchWarp<T, W, NORM, false, 1>(a, st);
-    if (groups <= kMaxThreads) return LaunchBlock<T, W, NORM, false, 1>(a, groups, st);
-    if (groups <= 4 * kMaxThreads) return LaunchBlock<T, W, NORM, false, 4>(a, groups, st);
+    // bf16 16384 x 4096 norm: 172 and 140 us with 1 and 2 groups; 8192 x 1003: 25 and 29 us
+    if (groups <= 256 || (!(NORM && many) && lanes <= kMaxThreads / 32 * 31)) return LaunchBlock<T, W, NORM, false, 1>(a, groups, st);
+    if (lanes <= kMaxThreads / 32 * 31 * 2) return LaunchBlock<T, W, NORM, false, 2>(a, groups, st);
+    if (lanes <= kMaxThreads / 32 * 31 * 4) return LaunchBlock<T, W, NORM, false, 4>(a, groups, st);
   }
   quant_long_rows_kernel<T, W, NORM><<<a.rows, kMaxThreads, 0, st>>>(a);
+}
+template <typename T, typename W, bool NORM>
+void LaunchAligned(const RowArgs& a, cudaStream_t st) {
+  auto at16 = [](const void* p, long long ld) { return (uintptr_t)p % 16 == 0 && ld * (long long)sizeof(T) % 16 == 0; };
+  const bool aligned = at16(a.x, a.ldx) && (uintptr_t)a.q % 8 == 0 && a.ldq % 8 == 0 &&
+                       (!NORM || ((!a.r || at16(a.r, a.ldr)) && (!a.h || at16(a.h, a.ldh)) && (uintptr_t)a.w % 16 == 0));
+  if (aligned) LaunchTW<T, W, NORM, true>(a, st);
+  else LaunchTW<T, W, NORM, false>(a, st);
 }
 
 template <typename T, bool NORM>
 void LaunchT(const RowArgs& a, int wtype, cudaStream_t st) {
-  if constexpr (!NORM) LaunchTW<T, float, NORM>(a, st);
-  else if (wtype == B200_DT_F32) LaunchTW<T, float, NORM>(a, st);
-  else if (wtype == B200_DT_BF16) LaunchTW<T, __nv_bfloat16, NORM>(a, st);
-  else LaunchTW<T, __half, NORM>(a, st);
+  if constexpr (!NORM) LaunchAligned<T, float, NORM>(a, st);
+  else if (wtype == B200_DT_F32) LaunchAligned<T, float, NORM>(a, st);
+  else if (wtype == B200_DT_BF16) LaunchAligned<T, __nv_bfloat16, NORM>(a, st);
+  else LaunchAligned<T, __half, NORM>(a, st);
 }
 
 template <bool NORM>
