@@ -51,40 +51,6 @@ struct Epilogue {
   int gelu;
 };
 
-// Two f32 operations in one instruction.
-struct F2 {
-  float x, y;
-};
-__device__ __forceinline__ uint64_t bits(F2 v) { return (uint64_t)__float_as_uint(v.y) << 32 | __float_as_uint(v.x); }
-__device__ __forceinline__ F2 floats(uint64_t b) { return {__uint_as_float((uint32_t)b), __uint_as_float((uint32_t)(b >> 32))}; }
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
-  return floats(d);
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
-  return floats(d);
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
-  return floats(d);
-}
-
-// Two integers as f32, rounded to nearest, without the conversion unit (a quarter of the rate and shared with
-// GELU's exponentials).  With H and L the halves of v + 2^31, the patterns 0x5300HHHH and 0x4b00LLLL are the
-// floats 2^39 + 2^16 H and 2^23 + L; taking 2^39 + 2^31 + 2^23 from the first is exact, and adding the second
-// rounds once.
-__device__ __forceinline__ F2 to_f32x2(int a, int b) {
-  constexpr float kOff = -(549755813888.f + 2147483648.f + 8388608.f);
-  const uint32_t u = (uint32_t)a ^ 0x80000000u, w = (uint32_t)b ^ 0x80000000u;
-  const F2 hi = {__uint_as_float(__byte_perm(u, 0x53000000u, 0x7632)), __uint_as_float(__byte_perm(w, 0x53000000u, 0x7632))};
-  const F2 lo = {__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7610)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7610))};
-  return add2(add2(hi, {kOff, kOff}), lo);
-}
-
 // The tanh form of GELU, 0.5 v (1 + tanh u) with u = sqrt(2 / pi) (v + 0.044715 v^3), as v / (1 + e^-2u):
 // the same function without the cancellation in 1 + tanh(u) for u < 0.
 __device__ __forceinline__ float gelu_tanh(float v) {
@@ -95,11 +61,10 @@ __device__ __forceinline__ float gelu_tanh(float v) {
   return v * r;
 }
 
-// act(f32(acc) * sa * sb + bias) of two sums.
-__device__ __forceinline__ F2 finish2(int a, int b, float sa, F2 sb, F2 bias, int gelu) {
-  F2 v = fma2(mul2(to_f32x2(a, b), {sa, sa}), sb, bias);
-  if (gelu) v = {gelu_tanh(v.x), gelu_tanh(v.y)};
-  return v;
+// act(f32(acc) * sa * sb + bias).
+__device__ __forceinline__ float finish(int acc, float sa, float sb, float bias, int gelu) {
+  const float v = fmaf((float)acc * sa, sb, bias);
+  return gelu ? gelu_tanh(v) : v;
 }
 
 __device__ __forceinline__ uint32_t pack2(int out, float lo, float hi) {
@@ -124,7 +89,7 @@ struct TileCfg {
   static constexpr int kStage = kABytes + kBBytes;
   // about 100 KB, so that two CTAs share an SM and one's loads run under the other's end
   static constexpr int kStages = BT == 32 ? 5 : BT == 64 ? 4 : 3;
-  static constexpr int kSmem = kStages * kStage + 1024 + 256 + BT * 4;
+  static constexpr int kSmem = kStages * kStage + 1024 + 256 + (BT + 256) * 4;
   static_assert(kStages * kStage >= BT * 128 * 4, "the sums of a tile lie over its stages");
 };
 
@@ -147,7 +112,9 @@ gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   uint64_t* empty = full + CF::kStages;
   uint64_t* acc_full = empty + CF::kStages;
   uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
-  float* sa_of = (float*)(smem + CF::kStages * CF::kStage + 256);   // the tile's token scales
+  float* sa_of = (float*)(smem + CF::kStages * CF::kStage + 256);
+  float* sb_of = sa_of + BT;
+  float* bias_of = sb_of + 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nb = (N + 127) / 128;
   const int rank = (int)(blockIdx.x % splits), tile = (int)(blockIdx.x / splits);
@@ -155,6 +122,12 @@ gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const int kbs = (K + BK - 1) / BK, kps = (kbs + splits - 1) / splits;
   const int kb0 = rank * kps, kb1 = min(kbs, kb0 + kps);   // never empty (the host picks `splits` so)
 
+  auto load = [&](int s, int kb) {
+    mbar_arrive_expect_tx(&full[s], CF::kStage);
+    uint8_t* st = smem + s * CF::kStage;
+    tma_load_2d_map(&tmB, &full[s], st, kb * BK, n0);
+    tma_load_2d_map(&tmA, &full[s], st + CF::kBBytes, kb * BK, t0);
+  };
   if (threadIdx.x == 0) {
     for (int s = 0; s < CF::kStages; ++s) {
       mbar_init(&full[s], 1);
@@ -162,6 +135,8 @@ gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     mbar_init(acc_full, 1);
     fence_barrier_init();
+    // the first loads run under the rest of the set-up
+    for (int s = 0; s < CF::kStages && kb0 + s < kb1; ++s) load(s, kb0 + s);
   }
   if (warp == 1) tmem_alloc(tmem_slot, BT);
   tc_fence_before();
@@ -169,35 +144,25 @@ gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // while the loads run: the scales and bias of this lane's four channels, and the tokens' scales
-  const int n = n0 + lane * 4;
-  F2 sb[2], bias[2];
-  auto channel = [&](const float* p, int j, float none) { return p && j < N ? p[j] : none; };
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    sb[e] = {channel(ep.b_scale, n + 2 * e, 1.f), channel(ep.b_scale, n + 2 * e + 1, 1.f)};
-    bias[e] = {channel(ep.bias, n + 2 * e, 0.f), channel(ep.bias, n + 2 * e + 1, 0.f)};
+  if (warp >= 2) {                               // while the loads run: the scales of the tile's rows, and its bias
+    const int e = threadIdx.x - 64, n = n0 + e;
+    sb_of[e] = ep.b_scale && n < N ? ep.b_scale[n] : 1.f;
+    bias_of[e] = ep.bias && n < N ? ep.bias[n] : 0.f;
+    if (e < BT) sa_of[e] = ep.a_scale && t0 + e < M ? ep.a_scale[t0 + e] : 1.f;
   }
-  if (warp >= 2)
-    for (int j = threadIdx.x - 64; j < BT; j += kThreads - 64) sa_of[j] = ep.a_scale && t0 + j < M ? ep.a_scale[t0 + j] : 1.f;
 
   if (warp == 0) {
     if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 0, issued = 0, fill_par = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      int s = 0, filled = min(CF::kStages, kb1 - kb0);
+      uint32_t ph = 1, fill_par = 0;             // of the stage's next fill; of its last
+      for (int kb = kb0 + CF::kStages; kb < kb1; ++kb) {
         if (!mbar_wait(&empty[s], ph ^ 1, kErrTimeoutEmpty, &g_tc_error_gemm_i8)) break;
-        mbar_arrive_expect_tx(&full[s], CF::kStage);
-        uint8_t* st = smem + s * CF::kStage;
-        tma_load_2d_map(&tmB, &full[s], st, kb * BK, n0);
-        tma_load_2d_map(&tmA, &full[s], st + CF::kBBytes, kb * BK, t0);
-        issued |= 1u << s;
+        load(s, kb);
         fill_par = (fill_par & ~(1u << s)) | (ph << s);
         if (++s == CF::kStages) { s = 0; ph ^= 1; }
       }
       // never leave, nor lay the sums over a stage, with TMA writes in flight
-      for (int q = 0; q < CF::kStages; ++q)
-        if (issued & (1u << q)) mbar_wait(&full[q], (fill_par >> q) & 1, kErrTimeoutOther, &g_tc_error_gemm_i8);
+      for (int q = 0; q < filled; ++q) mbar_wait(&full[q], (fill_par >> q) & 1, kErrTimeoutOther, &g_tc_error_gemm_i8);
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -244,37 +209,62 @@ gemm_i8_tile_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     tc_fence_after();
     tmem_dealloc(tmem, BT);
   }
-  // a warp per token: a lane adds and finishes four channels
+  // a warp per token, four tokens at a time: a lane adds and finishes four channels
+  constexpr int kWarps = kThreads / 32;
   const int per = (BT + splits - 1) / splits, j1 = min(min(BT, (rank + 1) * per), M - t0);
+  const int n = n0 + lane * 4;
+  auto sum_of = [&](const int* at) {
+    if (splits == 1) return *(const int4*)at;
+    int4 acc = make_int4(0, 0, 0, 0), p[4];
+#pragma unroll
+    for (int c0 = 0; c0 < 8; c0 += 4) {          // four CTAs' sums on their way at a time
+      if (c0 >= splits) break;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        p[c] = c0 + c < splits ? ld_cluster_v4(cluster_addr(at, c0 + c)) : make_int4(0, 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        acc.x += p[c].x; acc.y += p[c].y; acc.z += p[c].z; acc.w += p[c].w;
+      }
+    }
+    return acc;
+  };
   if (n < N) {
-#pragma unroll 4
-    for (int j = rank * per + warp; j < j1; j += kThreads / 32) {
-      int4 acc = make_int4(0, 0, 0, 0);
-      const int* at = sums + j * 128 + lane * 4;
-      if (splits == 1) {
-        acc = *(const int4*)at;
-      } else {
-        for (int c = 0; c < splits; ++c) {
-          const int4 p = ld_cluster_v4(cluster_addr(at, c));
-          acc.x += p.x; acc.y += p.y; acc.z += p.z; acc.w += p.w;
+    const float4 sb = *(const float4*)(sb_of + lane * 4), bias = *(const float4*)(bias_of + lane * 4);
+    for (int j0 = rank * per + warp; j0 < j1; j0 += 4 * kWarps) {
+      int4 acc[4];
+      float sa[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + u * kWarps;
+        if (j < j1) {
+          sa[u] = sa_of[j];
+          acc[u] = sum_of(sums + j * 128 + lane * 4);
         }
       }
-      const long long o = (long long)(t0 + j) * ldc + n;
-      F2 v[2] = {};
-      if (OUT != kOutS32) {
-        v[0] = finish2(acc.x, acc.y, sa_of[j], sb[0], bias[0], ep.gelu);
-        v[1] = finish2(acc.z, acc.w, sa_of[j], sb[1], bias[1], ep.gelu);
-      }
-      if (vec_store && n + 4 <= N) {
-        if (OUT == kOutS32) *(int4*)((int*)C + o) = acc;
-        else if (OUT == kOutF32) *(float4*)((float*)C + o) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-        else *(uint2*)((uint16_t*)C + o) = make_uint2(pack2(OUT, v[0].x, v[0].y), pack2(OUT, v[1].x, v[1].y));
-      } else {
-        const int a4[4] = {acc.x, acc.y, acc.z, acc.w};
-        const float v4[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < N) store_one<OUT>(C, o + e, a4[e], v4[e]);
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + u * kWarps;
+        if (j >= j1) break;
+        const long long o = (long long)(t0 + j) * ldc + n;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (OUT != kOutS32) {
+          v.x = finish(acc[u].x, sa[u], sb.x, bias.x, ep.gelu);
+          v.y = finish(acc[u].y, sa[u], sb.y, bias.y, ep.gelu);
+          v.z = finish(acc[u].z, sa[u], sb.z, bias.z, ep.gelu);
+          v.w = finish(acc[u].w, sa[u], sb.w, bias.w, ep.gelu);
+        }
+        if (vec_store && n + 4 <= N) {
+          if (OUT == kOutS32) *(int4*)((int*)C + o) = acc[u];
+          else if (OUT == kOutF32) *(float4*)((float*)C + o) = v;
+          else *(uint2*)((uint16_t*)C + o) = make_uint2(pack2(OUT, v.x, v.y), pack2(OUT, v.z, v.w));
+        } else {
+          const int a4[4] = {acc[u].x, acc[u].y, acc[u].z, acc[u].w};
+          const float v4[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < N) store_one<OUT>(C, o + e, a4[e], v4[e]);
+        }
       }
     }
   }
@@ -305,7 +295,6 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_read0() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // Bands of kGroupM token blocks, channel blocks inside a band: tiles worked on at the same time share operand
 // blocks in L2.
@@ -418,21 +407,36 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const int q = warp & 3, half = (warp - 2) >> 2;
     uint8_t* box = box_base + (warp - 2) * 4096;
     float* scales = (float*)(box_base + CF::kBox);
+    // This thread's part of a tile's scales: its row's, and those of one channel, which it hands to the others
+    // through shared memory.  Loaded a tile ahead: from HBM they take as long as half a tile.
+    struct Ahead {
+      float sa, sb, bias;
+    };
+    auto ahead = [&](int t) {
+      Ahead v = {1.f, 1.f, 0.f};
+      if (t >= tiles) return v;
+      int m_blk, n_blk;
+      pair_tile(t, mb, nb, &m_blk, &n_blk);
+      const int row = m_blk * 256 + (int)rank * 128 + q * 32 + lane, col = n_blk * CF::BN + (int)threadIdx.x - 64;
+      if (ep.a_scale && row < M) v.sa = ep.a_scale[row];
+      if (ep.b_scale && col < N) v.sb = ep.b_scale[col];
+      if (ep.bias && col < N) v.bias = ep.bias[col];
+      return v;
+    };
     int local = 0;
     bool ok = true;
+    Ahead next = ahead(pair);
     for (int t = pair; t < tiles; t += pairs, ++local) {
       const int a = local & 1;
       int m_blk, n_blk;
       pair_tile(t, mb, nb, &m_blk, &n_blk);
-      const int r0 = m_blk * 256 + (int)rank * 128 + q * 32, row = r0 + lane;   // this thread's token
+      const int r0 = m_blk * 256 + (int)rank * 128 + q * 32;       // the warp's first token
       float* sb_of = scales + a * 2 * CF::BN;
       float* bias_of = sb_of + CF::BN;
-      const float sa = ep.a_scale && row < M ? ep.a_scale[row] : 1.f;
-      {
-        const int j = threadIdx.x - 64, col = n_blk * CF::BN + j;
-        sb_of[j] = ep.b_scale && col < N ? ep.b_scale[col] : 1.f;
-        bias_of[j] = ep.bias && col < N ? ep.bias[col] : 0.f;
-      }
+      const float sa = next.sa;
+      sb_of[threadIdx.x - 64] = next.sb;
+      bias_of[threadIdx.x - 64] = next.bias;
+      next = ahead(t + pairs);
       // the eight warps' values are there; and, as every warp is past the tile before, its half may be
       // written again for the next.  A wait that gave up does not leave the loop: the others count on it here.
       asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -452,12 +456,9 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 sb = *(const float4*)(sb_of + c + j), bi = *(const float4*)(bias_of + c + j);
-            const F2 lo = finish2((int)v[j], (int)v[j + 1], sa, {sb.x, sb.y}, {bi.x, bi.y}, GELU);
-            const F2 hi = finish2((int)v[j + 2], (int)v[j + 3], sa, {sb.z, sb.w}, {bi.z, bi.w}, GELU);
-            v[j] = __float_as_uint(lo.x);
-            v[j + 1] = __float_as_uint(lo.y);
-            v[j + 2] = __float_as_uint(hi.x);
-            v[j + 3] = __float_as_uint(hi.y);
+            const float sb4[4] = {sb.x, sb.y, sb.z, sb.w}, bi4[4] = {bi.x, bi.y, bi.z, bi.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[j + e] = __float_as_uint(finish((int)v[j + e], sa, sb4[e], bi4[e], GELU));
           }
         }
         if (tma_store) {
@@ -503,7 +504,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       if (rank == 0) mbar_arrive(&acc_empty[a]);
       else mbar_arrive_remote(cluster_addr(&acc_empty[a], 0));
     }
-    if (lane == 0) bulk_wait_all();              // the stores complete before the shared memory goes away
+    if (lane == 0) bulk_wait_read0();            // the stores have read the shared memory before it goes away
   }
   __syncwarp();
   tc_fence_before();
@@ -512,6 +513,103 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, CF::kTmemCols);
   }
+}
+
+// ---------------------------------------------------------------------------------------- few tokens
+// 16 bytes at `p`, of which those at `end` and behind are not read from other lines than the row's own: the line
+// they lie in, or (not ALIGNED) the two lines, shifted together.  A line that holds a byte of the row lies in the
+// row's allocation.  What stands behind `end` in the last line remains in the result.
+template <bool ALIGNED>
+__device__ __forceinline__ uint4 load16(const int8_t* p, const int8_t* end) {
+  if (ALIGNED) return p < end ? *(const uint4*)p : make_uint4(0u, 0u, 0u, 0u);
+  const int off = (int)((uintptr_t)p & 15);
+  const int8_t* line = p - off;
+  const uint4 a = p < end ? *(const uint4*)line : make_uint4(0u, 0u, 0u, 0u);
+  const uint4 b = off && line + 16 < end ? *(const uint4*)(line + 16) : make_uint4(0u, 0u, 0u, 0u);
+  uint32_t x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) x[i] = off & 8 ? x[i + 2] : x[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) x[i] = off & 4 ? x[i + 1] : x[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = __funnelshift_r(x[i], x[i + 1], 8 * (off & 3));
+  return make_uint4(x[0], x[1], x[2], x[3]);
+}
+// The same with zeros from `end` on.
+template <bool ALIGNED>
+__device__ __forceinline__ uint4 load16_to(const int8_t* p, const int8_t* end) {
+  const uint4 v = load16<ALIGNED>(p, end);
+  const long long left = end - p;
+  if (left >= 16) return v;
+  uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int keep = (int)max(0ll, min(4ll, left - 4 * i));
+    x[i] = keep == 4 ? x[i] : x[i] & ((1u << (8 * keep)) - 1u);
+  }
+  return make_uint4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ int dot16(uint4 a, uint4 b, int acc) {
+  acc = __dp4a((int)a.x, (int)b.x, acc);
+  acc = __dp4a((int)a.y, (int)b.y, acc);
+  acc = __dp4a((int)a.z, (int)b.z, acc);
+  return __dp4a((int)a.w, (int)b.w, acc);
+}
+
+// Up to MT tokens: the weights' bytes bound it, and it starts faster than a pipeline of TMA and tensor core
+// (nothing to set up, sums in registers).  A warp takes R channels, its lanes 16 bytes of K each; `ks` of the
+// block's eight warps share the channels and cut K.
+template <int MT, int OUT, bool ALIGNED>
+__global__ void __launch_bounds__(256)
+gemv_i8_kernel(const int8_t* __restrict__ A, long long lda, const int8_t* __restrict__ B, long long ldb, void* __restrict__ C,
+               long long ldc, int M, int N, int K, int ks, const Epilogue ep) {
+  constexpr int R = MT <= 4 ? 4 : 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = warp % ks, n0 = (int)(blockIdx.x * (8 / ks) + warp / ks) * R;
+  // the lane's result: channel n0 + lane % R of token lane / R
+  const int n = n0 + lane % R, m = lane / R;
+  const bool mine = lane < R * MT && m < M && n < N;
+  float sa = 1.f, sb = 1.f, bias = 0.f;
+  if (mine && part == 0) {
+    if (ep.a_scale) sa = ep.a_scale[m];
+    if (ep.b_scale) sb = ep.b_scale[n];
+    if (ep.bias) bias = ep.bias[n];
+  }
+  int acc[R][MT] = {};
+  const int8_t* b_row[R];
+  const int8_t* a_row[MT];
+#pragma unroll
+  for (int r = 0; r < R; ++r) b_row[r] = B + (long long)min(n0 + r, N - 1) * ldb;
+#pragma unroll
+  for (int t = 0; t < MT; ++t) a_row[t] = A + (long long)min(t, M - 1) * lda;
+#pragma unroll 2
+  for (int k = (part * 32 + lane) * 16; k < K; k += ks * 512) {
+    uint4 b[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) b[r] = load16<ALIGNED>(b_row[r] + k, b_row[r] + K);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const uint4 a = load16_to<ALIGNED>(a_row[t] + k, a_row[t] + K);   // zeros behind K: b may hold anything there
+#pragma unroll
+      for (int r = 0; r < R; ++r) acc[r][t] = dot16(a, b[r], acc[r][t]);
+    }
+  }
+  int sum = 0;
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int v = __reduce_add_sync(0xffffffffu, acc[r][t]);
+      sum = lane == t * R + r ? v : sum;
+    }
+  if (ks > 1) {
+    __shared__ int s_sum[8][32];
+    s_sum[warp][lane] = sum;
+    __syncthreads();
+    if (part != 0) return;
+    for (int p = 1; p < ks; ++p) sum += s_sum[warp + p][lane];
+  }
+  if (mine) store_one<OUT>(C, (long long)m * ldc + n, sum, OUT == kOutS32 ? 0.f : finish(sum, sa, sb, bias, ep.gelu));
 }
 
 // ---------------------------------------------------------------------------------------- operands
@@ -547,7 +645,7 @@ __global__ void __launch_bounds__(256) no_depth_kernel(void* __restrict__ C, lon
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)M * N; i += (long long)gridDim.x * 256) {
     const long long m = i / N, n = i % N;
     const float sb = ep.b_scale ? ep.b_scale[n] : 1.f, bias = ep.bias ? ep.bias[n] : 0.f;
-    store_one<OUT>(C, m * ldc + n, 0, finish2(0, 0, ep.a_scale ? ep.a_scale[m] : 1.f, {sb, sb}, {bias, bias}, ep.gelu).x);
+    store_one<OUT>(C, m * ldc + n, 0, finish(0, ep.a_scale ? ep.a_scale[m] : 1.f, sb, bias, ep.gelu));
   }
 }
 
@@ -593,11 +691,14 @@ struct Call {
   cudaStream_t st;
 };
 
-// The launch form of a product: CTA pairs, or single tiles of `bt` tokens with K cut over `splits` CTAs.
+// The launch form of a product: CTA pairs, single tiles of `bt` tokens with K cut over `splits` CTAs, or (bt 0) sums
+// in registers with K cut over `splits` warps.
 struct Form {
   bool pair = false;
   int bt = 32, splits = 1;
+  bool tma() const { return pair || bt; }        // whether it reads its operands by TMA
 };
+constexpr int kGemvTokens = 8;                   // the most the last form takes
 
 int Launched(cudaError_t e) {
   if (e != cudaSuccess) {
@@ -655,7 +756,9 @@ template <int OUT, bool GELU>
 int LaunchPair(const Call& c) {
   CUtensorMap ta, tb, tc;
   if (!MakeI8Map(&ta, c.A, c.lda, c.M, c.K, 128) || !MakeI8Map(&tb, c.B, c.ldb, c.N, c.K, 128)) return -2;
-  const int tma_store = (uintptr_t)c.C % 16 == 0 && c.ldc * kOutBytes<OUT> % 16 == 0 && MakeOutMap(&tc, c.C, c.ldc, c.M, c.N, OUT);
+  // (a TMA store writes 16 bytes at least: columns up to the next multiple would be overwritten with zeros)
+  const int tma_store = (uintptr_t)c.C % 16 == 0 && c.ldc * kOutBytes<OUT> % 16 == 0 && (int64_t)c.N * kOutBytes<OUT> % 16 == 0 &&
+                        MakeOutMap(&tc, c.C, c.ldc, c.M, c.N, OUT);
   if (!tma_store) tc = ta;                       // unused
   const int64_t tiles = (int64_t)((c.M + 255) / 256) * ((c.N + 255) / 256);
   if (tiles > INT32_MAX / 2) return -1;
@@ -664,6 +767,19 @@ int LaunchPair(const Call& c) {
   const int pairs = (int)std::min<int64_t>(tiles, NumSMs() / 2);   // one CTA per SM
   return LaunchClusters(gemm_i8_pair_kernel<OUT, GELU>, 2 * pairs, PairCfg::kThreads, 2, PairCfg::kSmem, c.st, ta, tb, tc, c.C, (long long)c.ldc, c.M, c.N,
                         c.K, c.ep, tma_store);
+}
+
+template <int MT, int OUT>
+int LaunchGemv(const Call& c, int ks) {
+  constexpr int R = MT <= 4 ? 4 : 2;
+  const int per = 8 / ks * R;
+  const unsigned grid = (unsigned)((c.N + per - 1) / per);
+  const int8_t *a = (const int8_t*)c.A, *b = (const int8_t*)c.B;
+  if (TmaRows(c.A, c.lda) && TmaRows(c.B, c.ldb))
+    gemv_i8_kernel<MT, OUT, true><<<grid, 256, 0, c.st>>>(a, c.lda, b, c.ldb, c.C, c.ldc, c.M, c.N, c.K, ks, c.ep);
+  else
+    gemv_i8_kernel<MT, OUT, false><<<grid, 256, 0, c.st>>>(a, c.lda, b, c.ldb, c.C, c.ldc, c.M, c.N, c.K, ks, c.ep);
+  return Launched(cudaGetLastError());
 }
 
 template <int OUT>
@@ -681,6 +797,12 @@ int LaunchForm(const Call& c, const Form& f) {
   } else {
     if (f.pair) return c.ep.gelu ? LaunchPair<OUT, true>(c) : LaunchPair<OUT, false>(c);
   }
+  if (f.bt == 0) {
+    if (c.M == 1) return LaunchGemv<1, OUT>(c, f.splits);
+    if (c.M == 2) return LaunchGemv<2, OUT>(c, f.splits);
+    if (c.M <= 4) return LaunchGemv<4, OUT>(c, f.splits);
+    return LaunchGemv<8, OUT>(c, f.splits);
+  }
   if (f.bt == 32) return LaunchTile<32, OUT>(c, f.splits);
   if (f.bt == 64) return LaunchTile<64, OUT>(c, f.splits);
   return LaunchTile<128, OUT>(c, f.splits);
@@ -688,26 +810,40 @@ int LaunchForm(const Call& c, const Form& f) {
 
 Form ChooseForm(int64_t M, int64_t N, int64_t K, int sms) {
   Form f;
-  f.bt = M <= 32 ? 32 : M <= 64 ? 64 : 128;
   const int64_t kbs = (K + BK - 1) / BK;
-  const int64_t tiles = ((N + 127) / 128) * ((M + f.bt - 1) / f.bt);
-  const int64_t pair_tiles = ((M + 255) / 256) * ((N + 255) / 256);
-  f.pair = M >= 256 && pair_tiles * 2 >= sms;
-  for (int s = 8; s > 1; s /= 2) {
-    const int64_t kps = (kbs + s - 1) / s;
-    if (tiles * s <= 2 * sms && kps >= 2 && (s - 1) * kps < kbs) {
-      f.splits = s;
-      break;
+  if (M <= 2 || (M <= kGemvTokens && M * N * K <= 1 << 25)) {
+    f.bt = 0;
+    const int64_t warps = N / (M <= 4 ? 4 : 2);
+    while (f.splits < 8 && warps * f.splits < 4096 && f.splits * 512 < K) f.splits *= 2;
+  } else {
+    f.bt = M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    const int64_t tiles = ((N + 127) / 128) * ((M + f.bt - 1) / f.bt);
+    const int64_t pair_tiles = ((M + 255) / 256) * ((N + 255) / 256);
+    f.pair = M >= 256 && pair_tiles * 2 >= sms;
+    for (int s = 8; s > 1; s /= 2) {
+      const int64_t kps = (kbs + s - 1) / s;
+      if (tiles * s <= 2 * sms && kps >= 2 && (s - 1) * kps < kbs) {
+        f.splits = s;
+        break;
+      }
     }
   }
-  // B200_GEMM_I8_FORM = pair, or <tokens>x<splits>: every product in that form (for comparisons)
+  // B200_GEMM_I8_FORM = pair, <tokens>x<splits> or 0x<splits>: every product it fits in that form (for comparisons)
   if (const char* env = std::getenv("B200_GEMM_I8_FORM")) {
     int bt = 0, s = 0;
-    f.pair = env[0] == 'p';
-    if (!f.pair && std::sscanf(env, "%dx%d", &bt, &s) == 2 && (bt == 32 || bt == 64 || bt == 128) && s >= 1 && s <= 8) {
-      f.bt = bt;
-      for (f.splits = s; f.splits > 1; --f.splits)
-        if ((f.splits - 1) * ((kbs + f.splits - 1) / f.splits) < kbs) break;
+    if (env[0] == 'p') {
+      f.pair = true;
+    } else if (std::sscanf(env, "%dx%d", &bt, &s) == 2 && s >= 1 && s <= 8) {
+      if (bt == 32 || bt == 64 || bt == 128) {
+        f.pair = false;
+        f.bt = bt;
+        for (f.splits = s; f.splits > 1; --f.splits)
+          if ((f.splits - 1) * ((kbs + f.splits - 1) / f.splits) < kbs) break;
+      } else if (bt == 0 && M <= kGemvTokens && 8 % s == 0) {
+        f.pair = false;
+        f.bt = 0;
+        f.splits = s;
+      }
     }
   }
   return f;
@@ -727,7 +863,7 @@ int TakeGemmI8Error() {
 }
 
 size_t GemmI8ScratchBytes(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || !ChooseForm(M, N, K, NumSMs()).tma()) return 0;
   return PackedBytes(A, lda, M, K) + PackedBytes(B, ldb, N, K);
 }
 
@@ -742,7 +878,9 @@ int GemmI8(const void* A, int64_t lda, const void* B, int64_t ldb, const float* 
   if (M == 0 || N == 0) return 0;
   const int es = out == kOutBF16 || out == kOutF16 ? 2 : 4;
   if ((K && (!A || !B)) || !C || (uintptr_t)C % es || (uintptr_t)a_scale % 4 || (uintptr_t)b_scale % 4 || (uintptr_t)bias % 4) return -1;
-  const size_t need_a = K ? PackedBytes(A, lda, M, K) : 0, need_b = K ? PackedBytes(B, ldb, N, K) : 0;
+  const Form f = ChooseForm(M, N, K, NumSMs());
+  const bool tma = K && f.tma();
+  const size_t need_a = tma ? PackedBytes(A, lda, M, K) : 0, need_b = tma ? PackedBytes(B, ldb, N, K) : 0;
   if (need_a + need_b && (!scratch || need_a + need_b > scratch_bytes || (uintptr_t)scratch % 256)) return -4;
   Call c = {A, B, C, lda, ldb, ldc, (int)M, (int)N, (int)K, out, {a_scale, b_scale, bias, act}, st};
   if (need_a + need_b) {
@@ -769,7 +907,6 @@ int GemmI8(const void* A, int64_t lda, const void* B, int64_t ldb, const float* 
     pack_rows_kernel<<<(unsigned)std::min<long long>(blocks, NumSMs() * 16), 256, 0, st>>>(p);
     if (int rc = Launched(cudaGetLastError())) return rc;
   }
-  const Form f = ChooseForm(M, N, K, NumSMs());
   if (out == kOutF32) return LaunchForm<kOutF32>(c, f);
   if (out == kOutBF16) return LaunchForm<kOutBF16>(c, f);
   if (out == kOutF16) return LaunchForm<kOutF16>(c, f);

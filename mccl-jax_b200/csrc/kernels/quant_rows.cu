@@ -56,8 +56,16 @@ __device__ __forceinline__ __half add_rn(__half x, __half r) { return __hadd_rn(
 struct F2 {
   float x, y;
 };
-__device__ __forceinline__ uint64_t bits(F2 v) { return (uint64_t)__float_as_uint(v.y) << 32 | __float_as_uint(v.x); }
-__device__ __forceinline__ F2 floats(uint64_t b) { return {__uint_as_float((uint32_t)b), __uint_as_float((uint32_t)(b >> 32))}; }
+__device__ __forceinline__ uint64_t bits(F2 v) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(v.x), "f"(v.y));
+  return d;
+}
+__device__ __forceinline__ F2 floats(uint64_t b) {
+  F2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(b));
+  return v;
+}
 __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
   uint64_t d;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));

@@ -284,11 +284,12 @@ def test_gemm_sums(k, cuda, m, n, kk, pad, offset):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("form", ["pair", "32x1", "32x3", "32x8", "64x1", "64x4", "64x7", "128x1", "128x2", "128x5", "128x8"])
-@pytest.mark.parametrize("m,n,kk", [(1, 300, 1500), (70, 130, 1024), (300, 520, 1000), (515, 1031, 1280)])
+@pytest.mark.parametrize("form", ["pair", "0x1", "0x2", "0x4", "0x8", "32x1", "32x3", "32x8", "64x1", "64x4", "64x7", "128x1", "128x2", "128x5", "128x8"])
+@pytest.mark.parametrize("m,n,kk", [(1, 300, 1500), (2, 77, 4113), (3, 515, 768), (6, 129, 200), (8, 64, 999), (70, 130, 1024), (300, 520, 1000), (515, 1031, 1280)])
 @pytest.mark.parametrize("npad", [0, 3])
 def test_gemm_every_form(k, cuda, monkeypatch, form, m, n, kk, npad):
-    """CTA pairs, and single tiles of 32 to 128 tokens with K cut over up to 8 CTAs, whatever the size."""
+    """CTA pairs, single tiles of 32 to 128 tokens with K cut over up to 8 CTAs, whatever the size, and (0x: up to 8
+    tokens) sums in registers with K cut over warps."""
     torch = cuda
     monkeypatch.setenv("B200_GEMM_I8_FORM", form)
     g = torch.Generator(device="cuda").manual_seed(m + n + kk)
