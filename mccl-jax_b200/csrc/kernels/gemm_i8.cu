@@ -280,9 +280,11 @@ struct PairCfg {
   static constexpr int kABytes = 128 * BK, kBBytes = BN / 2 * BK;
   static constexpr int kStage = kABytes + kBBytes;
   static constexpr int kStages = 5;
-  static constexpr int kThreads = 64 + 256;      // TMA warp, MMA warp, eight epilogue warps
-  static constexpr int kBox = 8 * 4096;          // per epilogue warp: 32 rows x 128 bytes
-  static constexpr int kScales = 2 * 2 * BN * 4; // the tile's channel scales and biases, of two tiles in turn
+  static constexpr int kEpiWarps = 8;
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;   // TMA warp, MMA warp, epilogue warps
+  static constexpr int kCols = BN * 4 / kEpiWarps;       // of a tile, an epilogue warp's columns (of 32 rows)
+  static constexpr int kBox = kEpiWarps * 2048;          // per epilogue warp: 32 rows x 64 bytes
+  static constexpr int kScales = kEpiWarps * 2 * kCols * 4;   // its columns' scales and biases
   static constexpr int kSmem = kStages * kStage + 1024 + 1024 + kBox + kScales;
   static constexpr int kTmemCols = 2 * BN;
 };
@@ -335,7 +337,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 512);             // the epilogue threads of both CTAs
+      mbar_init(&acc_empty[a], 2 * CF::kEpiWarps);   // the epilogue warps of both CTAs
     }
     fence_barrier_init();
   }
@@ -402,50 +404,53 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       }
     }
   } else {
-    // A warp reads its quarter of the tile's rows and one half of its columns.  The quarter follows from the
-    // warp's number: it may access 32 of the 128 lanes of tensor memory.
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* box = box_base + (warp - 2) * 4096;
-    float* scales = (float*)(box_base + CF::kBox);
-    // This thread's part of a tile's scales: its row's, and those of one channel, which it hands to the others
-    // through shared memory.  Loaded a tile ahead: from HBM they take as long as half a tile.
+    // A warp reads a quarter of the tile's rows (which one follows from its number: it may access 32 of the 128
+    // lanes of tensor memory) and kCols of its columns, and shares nothing with the other warps.
+    const int q = warp & 3, c0 = ((warp - 2) >> 2) * CF::kCols;
+    uint8_t* box = box_base + (warp - 2) * 2048;
+    float* sb_of = (float*)(box_base + CF::kBox) + (warp - 2) * 2 * CF::kCols;
+    float* bias_of = sb_of + CF::kCols;
+    // This lane's part of a tile's scales: its row's, and those of the channels it hands to the warp through
+    // shared memory.  Loaded a tile ahead: from HBM they take as long as half a tile.
+    constexpr int kMine = CF::kCols / 32;
     struct Ahead {
-      float sa, sb, bias;
+      float sa, sb[kMine], bias[kMine];
     };
     auto ahead = [&](int t) {
-      Ahead v = {1.f, 1.f, 0.f};
-      if (t >= tiles) return v;
+      Ahead v;
       int m_blk, n_blk;
-      pair_tile(t, mb, nb, &m_blk, &n_blk);
-      const int row = m_blk * 256 + (int)rank * 128 + q * 32 + lane, col = n_blk * CF::BN + (int)threadIdx.x - 64;
-      if (ep.a_scale && row < M) v.sa = ep.a_scale[row];
-      if (ep.b_scale && col < N) v.sb = ep.b_scale[col];
-      if (ep.bias && col < N) v.bias = ep.bias[col];
+      pair_tile(min(t, tiles - 1), mb, nb, &m_blk, &n_blk);
+      const int row = m_blk * 256 + (int)rank * 128 + q * 32 + lane;
+      v.sa = ep.a_scale && row < M ? ep.a_scale[row] : 1.f;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int col = n_blk * CF::BN + c0 + 32 * i + lane;
+        v.sb[i] = ep.b_scale && col < N ? ep.b_scale[col] : 1.f;
+        v.bias[i] = ep.bias && col < N ? ep.bias[col] : 0.f;
+      }
       return v;
     };
     int local = 0;
-    bool ok = true;
     Ahead next = ahead(pair);
     for (int t = pair; t < tiles; t += pairs, ++local) {
       const int a = local & 1;
       int m_blk, n_blk;
       pair_tile(t, mb, nb, &m_blk, &n_blk);
       const int r0 = m_blk * 256 + (int)rank * 128 + q * 32;       // the warp's first token
-      float* sb_of = scales + a * 2 * CF::BN;
-      float* bias_of = sb_of + CF::BN;
       const float sa = next.sa;
-      sb_of[threadIdx.x - 64] = next.sb;
-      bias_of[threadIdx.x - 64] = next.bias;
+      __syncwarp();                              // the tile before is finished
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        sb_of[32 * i + lane] = next.sb[i];
+        bias_of[32 * i + lane] = next.bias[i];
+      }
       next = ahead(t + pairs);
-      // the eight warps' values are there; and, as every warp is past the tile before, its half may be
-      // written again for the next.  A wait that gave up does not leave the loop: the others count on it here.
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      ok = ok && mbar_wait_warp(&acc_full[a], (local >> 1) & 1, kErrTimeoutAcc, &g_tc_error_gemm_i8);
-      if (!ok) continue;
+      __syncwarp();
+      if (!mbar_wait_warp(&acc_full[a], (local >> 1) & 1, kErrTimeoutAcc, &g_tc_error_gemm_i8)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + a * CF::BN + ((uint32_t)(q * 32) << 16);
 #pragma unroll 1
-      for (int c = half * (CF::BN / 2); c < (half + 1) * (CF::BN / 2); c += 32) {
+      for (int c = c0; c < c0 + CF::kCols; c += 32) {
         const int col = n_blk * CF::BN + c;
         if (col >= N) break;                     // warp-uniform
         uint32_t v[32];
@@ -455,54 +460,59 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if (OUT != kOutS32) {
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
-            const float4 sb = *(const float4*)(sb_of + c + j), bi = *(const float4*)(bias_of + c + j);
+            const float4 sb = *(const float4*)(sb_of + c - c0 + j), bi = *(const float4*)(bias_of + c - c0 + j);
             const float sb4[4] = {sb.x, sb.y, sb.z, sb.w}, bi4[4] = {bi.x, bi.y, bi.z, bi.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[j + e] = __float_as_uint(finish((int)v[j + e], sa, sb4[e], bi4[e], GELU));
           }
         }
         if (tma_store) {
-          // rows of 128 bytes in a swizzled box of 32 rows, one TMA store for 32 four-byte or 64 two-byte
-          // columns: whole lines, and the tensor map clips the tails
-          constexpr int kW = 32 * kOutBytes<OUT> / 4;                      // 4-byte words of this chunk's row
-          const int part = kW == 16 ? (c / 32) & 1 : 0;
-          uint32_t w[kW];
+          // 64 bytes of 32 rows (32 two-byte or 16 four-byte columns) in a swizzled box, written by one TMA store:
+          // whole sectors, and the tensor map clips the tails
+          constexpr int kParts = kOutBytes<OUT> / 2, kPart = 32 / kParts;
 #pragma unroll
-          for (int j = 0; j < kW; ++j)
-            w[j] = kW == 32 ? v[j] : pack2(OUT, __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-          if (part == 0) {
+          for (int h = 0; h < kParts; ++h) {
+            if (h && col + h * kPart >= N) break;
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              w[j] = kParts == 2 ? v[h * 16 + j] : pack2(OUT, __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
             if (lane == 0) bulk_wait_read0();    // the previous store has read the box
             __syncwarp();
-          }
 #pragma unroll
-          for (int i = 0; i < kW / 4; ++i)
-            *(uint4*)(box + lane * 128 + (((i + part * 4) ^ (lane & 7)) << 4)) =
-                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-          if (kW == 32 || part == 1 || col + 32 >= N) {
+            for (int i = 0; i < 4; ++i)
+              *(uint4*)(box + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_2d(&tmC, box, col - part * 32, r0);
+              tma_store_2d(&tmC, box, col + h * kPart, r0);
               bulk_commit();
             }
           }
         } else {
-          // rows of C that TMA cannot write: 32 x 32 results through shared memory, stored row by row
+          // rows of C that TMA cannot write: sixteen columns at a time through shared memory, two rows a store
           uint32_t* stage = (uint32_t*)box;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) stage[lane * 32 + (j ^ lane)] = v[j];
-          __syncwarp();
-#pragma unroll 4
-          for (int rr = 0; rr < 32; ++rr) {
-            const uint32_t x = stage[rr * 32 + (lane ^ rr)];
-            if (r0 + rr < M && col + lane < N) store_one<OUT>(C, (long long)(r0 + rr) * ldc + col + lane, (int)x, __uint_as_float(x));
+          for (int h = 0; h < 2; ++h) {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) stage[lane * 16 + (j ^ (lane >> 1 & 15))] = v[h * 16 + j];
+            __syncwarp();
+#pragma unroll
+            for (int rr = 0; rr < 32; rr += 2) {
+              const int r = rr + (lane >> 4), j = lane & 15, n = col + h * 16 + j;
+              const uint32_t x = stage[r * 16 + (j ^ (r >> 1 & 15))];
+              if (r0 + r < M && n < N) store_one<OUT>(C, (long long)(r0 + r) * ldc + n, (int)x, __uint_as_float(x));
+            }
           }
-          __syncwarp();
         }
       }
       tc_fence_before();
-      if (rank == 0) mbar_arrive(&acc_empty[a]);
-      else mbar_arrive_remote(cluster_addr(&acc_empty[a], 0));
+      __syncwarp();
+      if (lane == 0) {
+        if (rank == 0) mbar_arrive(&acc_empty[a]);
+        else mbar_arrive_remote_relaxed(cluster_addr(&acc_empty[a], 0));
+      }
     }
     if (lane == 0) bulk_wait_read0();            // the stores have read the shared memory before it goes away
   }
@@ -666,18 +676,18 @@ bool MakeI8Map(CUtensorMap* map, const void* p, int64_t ld, int rows, int K, int
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// 2-D map over C for the pair kernel's stores: boxes of 32 rows x 128 bytes, 128-byte swizzle.
+// 2-D map over C for the pair kernel's stores: boxes of 32 rows x 64 bytes, 64-byte swizzle.
 bool MakeOutMap(CUtensorMap* map, void* C, int64_t ldc, int M, int N, int out) {
   EncodeTiledFn enc = GetEncodeTiled();
   if (!enc) return false;
   const int es = out == kOutBF16 || out == kOutF16 ? 2 : 4;
   cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
   cuuint64_t strides[1] = {(cuuint64_t)ldc * es};
-  cuuint32_t box[2] = {(cuuint32_t)(128 / es), 32}, estr[2] = {1, 1};
+  cuuint32_t box[2] = {(cuuint32_t)(64 / es), 32}, estr[2] = {1, 1};
   const CUtensorMapDataType t = out == kOutF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                               : out == kOutS32 ? CU_TENSOR_MAP_DATA_TYPE_INT32
                               : out == kOutBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  return enc(map, t, 2, C, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  return enc(map, t, 2, C, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

@@ -221,6 +221,11 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
+// The same without release: for a thread whose arrival hands over nothing it wrote (tensor memory that it has
+// finished reading).  The releasing form waits for the thread's earlier stores first.
+__device__ __forceinline__ void mbar_arrive_remote_relaxed(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
 // Tiled TMA load into this CTA's shared memory whose completion is counted on an mbarrier that may sit
 // in the peer CTA of the pair (`cluster_bar`, a shared::cluster address).  No multicast.
 __device__ __forceinline__ void tma_load_3d_pair(const CUtensorMap* map, uint32_t cluster_bar, void* dst, int c0, int c1, int c2) {
