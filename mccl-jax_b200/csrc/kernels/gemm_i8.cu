@@ -818,6 +818,16 @@ int LaunchForm(const Call& c, const Form& f) {
   return LaunchTile<128, OUT>(c, f.splits);
 }
 
+// Sums in registers for one or two tokens, and for up to eight where the products are few: a warp's dot products
+// go at 64 multiplies of four bytes a cycle and SM, so with more tokens they, not the weights' bytes, set the time
+// (8 x 2304 x 768: 3.3 us against 5.0 on the tensor core; 8 x 4096 x 4096: 15.5 against 8.3).  Their K is cut until
+// 4096 warps are at work.
+//
+// Otherwise the form that a model of the launch's time calls shortest, in microseconds on B200: a tile's CTA takes
+// `fixed` plus `block` for each 128 of K, and half of that again for each further CTA its SM holds (two at a time
+// share its loads); adding 2^i slices of K costs 0.76 i; pairs take 7.5 plus 0.333 for each round and 128 of K.
+// Fitted to the times of 13 forms at 37 sizes from 4 x 1000 x 1000 to 8192 x 768 x 768 and 1024 x 8192 x 8192: the
+// form it picks takes 4 % longer than the best of the 13 on average.
 Form ChooseForm(int64_t M, int64_t N, int64_t K, int sms) {
   Form f;
   const int64_t kbs = (K + BK - 1) / BK;
@@ -826,17 +836,28 @@ Form ChooseForm(int64_t M, int64_t N, int64_t K, int sms) {
     const int64_t warps = N / (M <= 4 ? 4 : 2);
     while (f.splits < 8 && warps * f.splits < 4096 && f.splits * 512 < K) f.splits *= 2;
   } else {
-    f.bt = M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    const int64_t tiles = ((N + 127) / 128) * ((M + f.bt - 1) / f.bt);
-    const int64_t pair_tiles = ((M + 255) / 256) * ((N + 255) / 256);
-    f.pair = M >= 256 && pair_tiles * 2 >= sms;
-    for (int s = 8; s > 1; s /= 2) {
-      const int64_t kps = (kbs + s - 1) / s;
-      if (tiles * s <= 2 * sms && kps >= 2 && (s - 1) * kps < kbs) {
-        f.splits = s;
-        break;
+    auto rounds = [](int64_t n, int64_t slots) { return (double)((n + slots - 1) / slots); };
+    double best = 1e300;
+    auto consider = [&](double t, bool pair, int bt, int splits) {
+      if (t >= best) return;
+      best = t;
+      f.pair = pair;
+      f.bt = bt;
+      f.splits = splits;
+    };
+    struct {
+      int bt;
+      double block, fixed;
+    } const tiles[] = {{32, 0.288, 4.2}, {64, 0.328, 4.8}, {128, 0.428, 6.1}};
+    for (const auto& tile : tiles)
+      for (int s = 1, i = 0; s <= 8; s *= 2, ++i) {
+        const int64_t kps = (kbs + s - 1) / s;
+        if (s > 1 && (s - 1) * kps >= kbs) break;          // a CTA without work
+        const int64_t ctas = ((N + 127) / 128) * ((M + tile.bt - 1) / tile.bt) * s;
+        const double per_sm = ctas <= 2 * sms ? std::max(1.0, (double)ctas / sms) : 2.0 * rounds(ctas, 2 * sms);
+        consider(0.76 * i + (tile.block * kps + tile.fixed) * 0.5 * (1.0 + per_sm), false, tile.bt, s);
       }
-    }
+    consider(7.5 + rounds(((M + 255) / 256) * ((N + 255) / 256), sms / 2) * 0.333 * kbs, true, 128, 1);
   }
   // B200_GEMM_I8_FORM = pair, <tokens>x<splits> or 0x<splits>: every product it fits in that form (for comparisons)
   if (const char* env = std::getenv("B200_GEMM_I8_FORM")) {
