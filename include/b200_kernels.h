@@ -54,7 +54,7 @@ B200_API int b200_gemm_split(const void* A, int a_type, const void* B, int b_typ
  * each (of activations: a scale per token; of a weight matrix [N, K]: a scale per output channel), and
  * b200_gemm_i8 multiplies two such operands.  Row pitches ld* count elements of their own array; rows
  * may start at any element, and those whose addresses and pitches are multiples of 16 bytes (q: 8) are
- * read and written fastest.  Bytes between a row's end and the next row are neither read nor written.
+ * read and written fastest.  Bytes between a row's end and the next row are not written.
  * All three only queue work on `stream`, which with every pointer belongs to the current device, and
  * may be captured.  They return 0, -1 (bad arguments), -2 (no tensor map), -3 (launch failure), or -4
  * (scratch too small or misaligned).  No counterpart in the reference, whose products are floating. */
@@ -69,7 +69,7 @@ B200_API int b200_quantize_i8(const void* x, int64_t ldx, int8_t* q, int64_t ldq
  * dtype (h = x without one), t = f32(h * weight), q = round_half_even(127 t / max_j |t|) as above, scale =
  * max_j |t| / 127 / sqrt(mean_j h^2 + eps), so the normalised row is about q * scale.  weight [cols] of
  * weight_dtype; x, residual and h of dtype, each in {F32, BF16, F16}.  residual may be NULL, and then h is
- * NULL too; with a residual h may be NULL (not written), or x or residual themselves with their pitch.
+ * NULL too; with a residual h may be NULL (not written), or x or residual themselves with their pitch (no other overlap).
  * eps > 0.  A row whose t holds an infinity or a NaN gives scale NaN and q 0.  rows may be 0. */
 B200_API int b200_rms_norm_i8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* h,
                               int64_t ldh, int8_t* q, int64_t ldq, float* scale, int64_t rows, int64_t cols, int dtype,
@@ -80,8 +80,9 @@ B200_API int b200_rms_norm_i8(const void* x, int64_t ldx, const void* residual, 
  * act B200_ACT_NONE or B200_ACT_GELU (its tanh form).  a_scale [M], b_scale [N] and bias [N] are f32 and may
  * each be NULL (1, 1, 0).  out_type S32 gives the sums themselves, without scales, bias or act.  Any of M, N,
  * K may be 0.  An operand whose address or pitch is no multiple of 16 bytes is first copied to such rows in
- * `scratch`, 256-byte aligned device memory of b200_gemm_i8_scratch_bytes(...) bytes for these operands (0
- * when both lie so: scratch may be NULL); calls that overlap on the GPU need a scratch each. */
+ * `scratch`, 256-byte aligned device memory of b200_gemm_i8_scratch_bytes(...) bytes for these operands (0, and
+ * scratch may be NULL, when both lie so, and for the few tokens that are multiplied where they lie); calls that
+ * overlap on the GPU need a scratch each.  A, B and C do not overlap. */
 #define B200_ACT_NONE 0
 #define B200_ACT_GELU 1
 B200_API size_t b200_gemm_i8_scratch_bytes(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N,

@@ -18,6 +18,7 @@
 #include <map>
 #include <set>
 #include <sstream>
+#include <tuple>
 #include <unordered_map>
 #include <unordered_set>
 
@@ -3556,6 +3557,7 @@ class Lowerer {
     g.N = prod(b, rf);
     g.K = prod(a, lc);
     DT at = StoredDt(a), bt = StoredDt(b);
+    if (at == DT::kS8 && bt == DT::kS8 && r->type.dt == DT::kS32) return EmitDotI8(op, g, lb, lf, lc, rb, rf, rc);
     if (!DTIsFloat(at) || !DTIsFloat(bt)) throw LowerError{"dot_general on non-float operands is not supported"};
     if (at == DT::kF64 || bt == DT::kF64) throw LowerError{"dot_general on f64 operands is not supported"};
     g.out = r->type.dt;
@@ -3670,6 +3672,42 @@ class Lowerer {
                (g.split ? " f32-split" : g.ab == DT::kF32 ? " f32-simt" : "");
     p_->steps.push_back(st);
     RecordDt(g.c, StoredDt(r));
+  }
+
+  // dot_general of 8-bit integers with 32-bit sums (g: its sizes): the integer tensor cores, on operands in
+  // [batch, rows, K] order whose rows TMA can read; others are copied to such rows first.
+  void EmitDotI8(Op* op, GemmStep g, const std::vector<int64_t>& lb, const std::vector<int64_t>& lf,
+                 const std::vector<int64_t>& lc, const std::vector<int64_t>& rb, const std::vector<int64_t>& rf,
+                 const std::vector<int64_t>& rc) {
+    if (g.K > b200k::kGemmI8MaxK)
+      throw LowerError{"dot_general on 8-bit integers sums at most " + std::to_string(b200k::kGemmI8MaxK) + " products"};
+    const int64_t pitch = (g.K + 15) / 16 * 16;
+    auto operand = [&](const Value* v, std::vector<int64_t> order, const std::vector<int64_t>& fr,
+                       const std::vector<int64_t>& ct) -> std::pair<int, int64_t> {
+      order.insert(order.end(), fr.begin(), fr.end());
+      order.insert(order.end(), ct.begin(), ct.end());
+      bool in_order = true;
+      for (size_t k = 0; k < order.size(); ++k) in_order = in_order && order[k] == (int64_t)k;
+      if (in_order && g.K == pitch) return {SlotFor(v), g.K};
+      // one row of K after the other, K as the innermost dimension also where it is several of v's or none
+      std::vector<int> perm(order.begin(), order.end());
+      std::vector<int64_t> dims;
+      for (int k : perm) dims.push_back(v->type.dims[k]);
+      if (ct.size() == 1 || g.K == pitch) return {EmitPermute(v, perm, dims, DT::kS8, ct.size() == 1 ? pitch : 0), ct.size() == 1 ? pitch : g.K};
+      throw LowerError{"dot_general on 8-bit integers: contracting " + std::to_string(ct.size()) +
+                       " dimensions of together " + std::to_string(g.K) + " elements (no multiple of 16)"};
+    };
+    std::tie(g.a, g.lda) = operand(op->operands[0], lb, lf, lc);
+    std::tie(g.b, g.ldb) = operand(op->operands[1], rb, rf, rc);
+    g.ab = g.a_dt = g.b_dt = DT::kS8;
+    g.out = DT::kS32;
+    g.c = SlotFor(op->result());
+    Step st;
+    st.kind = StepKind::kGemm;
+    st.gemm = g;
+    st.label = "gemm b" + std::to_string(g.batch) + " " + std::to_string(g.M) + "x" + std::to_string(g.N) + "x" + std::to_string(g.K) + " i8";
+    p_->steps.push_back(st);
+    RecordDt(g.c, DT::kS32);
   }
 
   void EmitAttention(Op* d2) {

@@ -648,6 +648,15 @@ std::string Executable::Run(DeviceState& dev, const std::vector<const void*>& ar
           const GemmStep& g = S.gemm;
           for (int s : {g.a, g.b, g.c, g.ws, g.split_ws}) { err = slot(s); if (!err.empty()) return fail(err); }
           const long long lda = g.lda ? g.lda : (g.a_mn ? g.M : g.K), ldb = g.ldb ? g.ldb : (g.b_mn ? g.N : g.K);
+          if (g.ab == DT::kS8) {                   // sums of 8-bit integers, one batch entry after the other
+            for (int64_t e = 0; e < g.batch; ++e) {
+              const int rc = b200k::GemmI8((const int8_t*)ptr[g.a] + e * g.M * lda, lda, (const int8_t*)ptr[g.b] + e * g.N * ldb, ldb,
+                                           nullptr, nullptr, nullptr, (int32_t*)ptr[g.c] + e * g.M * g.N, g.N, g.M, g.N, g.K,
+                                           PjrtType(g.out), B200_ACT_NONE, nullptr, 0, st);
+              if (rc != 0) return fail("gemm launch failed (" + std::to_string(rc) + ") for " + S.label);
+            }
+            break;
+          }
           int* counter = pd->gemm_counters ? pd->gemm_counters + pd->gemm_slot[i] : nullptr;
           int rc = g.split
               ? b200k::GemmSplit(ptr[g.a], lda, g.a_mn, PjrtType(g.a_dt), ptr[g.b], ldb, g.b_mn, PjrtType(g.b_dt), ptr[g.c],

@@ -57,15 +57,17 @@ def test_gemm_refusals(k, change):
     refused(lambda: k.gemm_i8(**{**a, **change}))
 
 
-@pytest.mark.parametrize("change,need", [({}, 0), (dict(a=P + 1), 8 * 48), (dict(lda=33), 8 * 48), (dict(b=P + 8), 16 * 48),
-                                         (dict(lda=33, ldb=34), 24 * 48)])
+@pytest.mark.parametrize("change,need", [({}, 0), (dict(a=P + 1), 100 * 48), (dict(lda=33), 100 * 48), (dict(b=P + 8), 1000 * 48),
+                                         (dict(lda=33, ldb=34), 1100 * 48), (dict(lda=33, ldb=34, m=2), 0)])
 def test_gemm_scratch(k, change, need):
-    """Operands that do not lie 16-byte aligned need room for copies, each rounded up to 256 bytes."""
-    a = {**dict(a=P, lda=48, b=P, ldb=48, m=8, n=16, k=33), **change}
-    room = sum((r * 48 + 255) // 256 * 256 for r, moved in ((8, a["a"] % 16 or a["lda"] % 16), (16, a["b"] % 16 or a["ldb"] % 16)) if moved)
+    """Operands that do not lie 16-byte aligned need room for copies, each rounded up to 256 bytes; one or two tokens
+    are multiplied where they lie."""
+    a = {**dict(a=P, lda=48, b=P, ldb=48, m=100, n=1000, k=33), **change}
+    moved = [(a["m"], a["a"] % 16 or a["lda"] % 16), (a["n"], a["b"] % 16 or a["ldb"] % 16)] if a["m"] > 2 else []
+    room = sum((r * 48 + 255) // 256 * 256 for r, copy in moved if copy)
     assert k.gemm_i8_scratch_bytes(**a) == room >= need
     if room:
-        call = dict(a_scale=None, b_scale=None, bias=None, c=P, ldc=16, out_type=BF16)
+        call = dict(a_scale=None, b_scale=None, bias=None, c=P, ldc=1000, out_type=BF16)
         refused(lambda: k.gemm_i8(**a, **call), -4)
         refused(lambda: k.gemm_i8(**a, **call, scratch=P, scratch_bytes=room - 1), -4)
         refused(lambda: k.gemm_i8(**a, **call, scratch=P + 16, scratch_bytes=room + 256), -4)
