@@ -55,6 +55,7 @@ B200_API int b200_gemm_split(const void* A, int a_type, const void* B, int b_typ
  * b200_gemm_i8 multiplies two such operands.  Row pitches ld* count elements of their own array; rows
  * may start at any element, and those whose addresses and pitches are multiples of 16 bytes (q: 8) are
  * read and written fastest.  Bytes between a row's end and the next row are not written.
+ * Outputs overlap no input but as said.
  * All three only queue work on `stream`, which with every pointer belongs to the current device, and
  * may be captured.  They return 0, -1 (bad arguments), -2 (no tensor map), -3 (launch failure), or -4
  * (scratch too small or misaligned).  No counterpart in the reference, whose products are floating. */
@@ -82,7 +83,7 @@ B200_API int b200_rms_norm_i8(const void* x, int64_t ldx, const void* residual, 
  * K may be 0.  An operand whose address or pitch is no multiple of 16 bytes is first copied to such rows in
  * `scratch`, 256-byte aligned device memory of b200_gemm_i8_scratch_bytes(...) bytes for these operands (0, and
  * scratch may be NULL, when both lie so, and for the few tokens that are multiplied where they lie); calls that
- * overlap on the GPU need a scratch each.  A, B and C do not overlap. */
+ * overlap on the GPU need a scratch each.  C overlaps neither operand. */
 #define B200_ACT_NONE 0
 #define B200_ACT_GELU 1
 B200_API size_t b200_gemm_i8_scratch_bytes(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N,

