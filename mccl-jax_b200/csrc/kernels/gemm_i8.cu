@@ -494,19 +494,35 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             }
           }
         } else {
-          // rows of C that TMA cannot write: sixteen columns at a time through shared memory, two rows a store
+          // rows of C that TMA cannot write: through shared memory, so that a store covers neighbours of one row
+          // (two-byte results, 32 columns) or of two (four-byte ones, 16 columns at a time)
+          const int rows = min(32, M - r0);
           uint32_t* stage = (uint32_t*)box;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          if constexpr (kOutBytes<OUT> == 2) {
             __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) stage[lane * 16 + (j ^ (lane >> 1 & 15))] = v[h * 16 + j];
+            for (int j = 0; j < 16; ++j)
+              stage[lane * 16 + (j ^ (lane >> 1 & 15))] = pack2(OUT, __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
             __syncwarp();
+            uint16_t* out = (uint16_t*)C + (long long)r0 * ldc + col + lane;
+            if (col + lane < N) {
+#pragma unroll 8
+              for (int r = 0; r < rows; ++r, out += ldc)
+                *out = ((const uint16_t*)box)[2 * (r * 16 + (lane >> 1 ^ (r >> 1 & 15))) + (lane & 1)];
+            }
+          } else {
 #pragma unroll
-            for (int rr = 0; rr < 32; rr += 2) {
-              const int r = rr + (lane >> 4), j = lane & 15, n = col + h * 16 + j;
-              const uint32_t x = stage[r * 16 + (j ^ (r >> 1 & 15))];
-              if (r0 + r < M && n < N) store_one<OUT>(C, (long long)(r0 + r) * ldc + n, (int)x, __uint_as_float(x));
+            for (int h = 0; h < 2; ++h) {
+              __syncwarp();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) stage[lane * 16 + (j ^ (lane >> 1 & 15))] = v[h * 16 + j];
+              __syncwarp();
+              const int j = lane & 15, n = col + h * 16 + j;
+              uint32_t* out = (uint32_t*)C + (long long)(r0 + (lane >> 4)) * ldc + n;
+              if (n < N) {
+#pragma unroll 8
+                for (int r = lane >> 4; r < rows; r += 2, out += 2 * ldc) *out = stage[r * 16 + (j ^ (r >> 1 & 15))];
+              }
             }
           }
         }
