@@ -518,7 +518,7 @@ void LaunchWarp(const RowArgs& a, cudaStream_t st) {
 template <typename T, typename W, bool NORM, bool ALIGNED>
 void LaunchTW(const RowArgs& a, cudaStream_t st) {
   const bool many = a.rows >= 148 * 8;
-  const int groups = (a.cols + 7) / 8;
+  const int groups = (int)((a.cols + 7ll) / 8);
   const int lanes = groups + (ALIGNED ? 0 : 1);  // see LaunchBlock
   if (lanes <= 8) return LaunchWarp<T, W, NORM, ALIGNED, 1, 8>(a, st);
   if (lanes <= 16) return LaunchWarp<T, W, NORM, ALIGNED, 1, 16>(a, st);

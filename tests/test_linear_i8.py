@@ -185,6 +185,21 @@ def test_quantize_no_columns(k, cuda):
     assert scale.tolist() == [0.0, 0.0, 0.0]
 
 
+@pytest.mark.gpu
+def test_quantize_longest_row(k, cuda):
+    """The longest row there may be, whose last group of eight ends past 2^31."""
+    torch = cuda
+    cols = (1 << 31) - 1
+    x = torch.empty(cols, device="cuda", dtype=torch.bfloat16).normal_(generator=torch.Generator(device="cuda").manual_seed(6))
+    x[cols - 1] = 50.0
+    q, scale = torch.full((cols,), 99, device="cuda", dtype=torch.int8), torch.empty(1, device="cuda")
+    k.quantize_i8(x.data_ptr(), cols, q.data_ptr(), cols, scale.data_ptr(), 1, cols, BF16, stream(torch))
+    for at in range(0, cols, 1 << 27):
+        part = x[at:at + (1 << 27)]
+        assert torch.equal(q[at:at + (1 << 27)], (part.double() * 127.0 / 50.0).round().to(torch.int8))
+    close_f32(torch, scale, torch.full((1,), 50.0, device="cuda").double() / 127.0, 1)
+
+
 # ------------------------------------------------------------------------------------------ norm
 def norm_reference(torch, x, r, w, eps):
     """(h, q, scale) in 64 bits, from h as it is stored."""
