@@ -326,7 +326,7 @@ __device__ __forceinline__ float row_scale(uint32_t mx, float ss, float down, in
   if (mx >= kInfBits) return __uint_as_float(0x7fc00000u);
   const float s = __uint_as_float(mx) / 127.0f;
   if (!NORM) return s;
-  return s * (1.0f / sqrtf(ss / (float)n + (down == 1.f ? eps : 0.f)) * down);   // (eps vanishes beside such squares)
+  return s * (1.0f / sqrtf(ss / (float)n + eps * down * down) * down);
 }
 
 // One row per LANES lanes of a warp, or (LANES 0) per block; each thread keeps NG groups of eight neighbours in

@@ -266,6 +266,28 @@ def test_rms_norm_rows_that_are_special(k, cuda, cols):
     close_f32(torch, scale, ref_scale, (math.log2(cols) + 34) / 2 + 4)
 
 
+def check_norm_f32(torch, k, x, w, eps):
+    """A norm of f32 rows whose residual is zero, q and h equal and the scale within the roundings of a sum of squares
+    (as in test_rms_norm)."""
+    rows, cols = x.shape
+    r = torch.zeros_like(x)
+    h, q, scale = torch.empty_like(x), torch.empty(rows, cols, device="cuda", dtype=torch.int8), torch.empty(rows, device="cuda")
+    ref_h, ref_q, ref_scale = norm_reference(torch, x, r, w, eps)
+    k.rms_norm_i8(x.data_ptr(), cols, r.data_ptr(), cols, w.data_ptr(), h.data_ptr(), cols, q.data_ptr(), cols, scale.data_ptr(), rows,
+                  cols, F32, F32, eps, stream(torch))
+    assert torch.equal(h, ref_h) and torch.equal(q, ref_q)
+    close_f32(torch, scale, ref_scale, (math.log2(cols) + 34) / 2 + 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [16, 1001, 6000, 40000])
+def test_rms_norm_large_eps(k, cuda, cols):
+    """An eps of the size of squares whose sum overflows, and beside smaller ones."""
+    torch = cuda
+    u = 0.5 + torch.rand(2, cols, device="cuda", generator=torch.Generator(device="cuda").manual_seed(8))
+    check_norm_f32(torch, k, u * torch.tensor([[1.5e19], [1e18]], device="cuda"), torch.ones(cols, device="cuda"), 3e38)
+
+
 # ------------------------------------------------------------------------------------------ gemm
 def operand(torch, g, rows, cols, pad, offset=0):
     v, _ = rows_of(torch, rows, cols, pad, torch.int8, fill=77, offset=offset)
