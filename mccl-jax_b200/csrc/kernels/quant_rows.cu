@@ -33,6 +33,7 @@ constexpr uint32_t kInfBits = 0x7f800000u;
 constexpr float kBorder = 0.5f - 1.0f / 16384.0f;
 constexpr float kRoundMagic = 12582912.0f;     // 1.5 * 2^23: adding it rounds |v| < 2^22 to an integer
 constexpr float kDown = 1.262177448353619e-29f;    // 2^-96
+constexpr float kSmall = 1.5046327690525280e-36f;  // 2^-119, just above 127 * 2^-126
 constexpr int kMaxThreads = 1024;
 
 struct RowArgs {
@@ -324,9 +325,11 @@ __device__ __forceinline__ RowRound row_round(uint32_t mx) {
 template <bool NORM>
 __device__ __forceinline__ float row_scale(uint32_t mx, float ss, float down, int n, float eps) {
   if (mx >= kInfBits) return __uint_as_float(0x7fc00000u);
-  const float s = __uint_as_float(mx) / 127.0f;
-  if (!NORM) return s;
-  return s * (1.0f / sqrtf(ss / (float)n + eps * down * down) * down);
+  const float m = __uint_as_float(mx);
+  if (!NORM) return m / 127.0f;
+  const float f = 1.0f / sqrtf(ss / (float)n + eps * down * down) * down;
+  // an m / 127 below the normal range has lost bits that a large f would bring back into the scale
+  return m < kSmall ? m * f / 127.0f : m / 127.0f * f;
 }
 
 // One row per LANES lanes of a warp, or (LANES 0) per block; each thread keeps NG groups of eight neighbours in

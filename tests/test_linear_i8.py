@@ -288,6 +288,15 @@ def test_rms_norm_large_eps(k, cuda, cols):
     check_norm_f32(torch, k, u * torch.tensor([[1.5e19], [1e18]], device="cuda"), torch.ones(cols, device="cuda"), 3e38)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [16, 1001, 6000, 40000])
+def test_rms_norm_small_products(k, cuda, cols):
+    """Values and weights whose products leave the normal range, under an eps that brings the scale back into it."""
+    torch = cuda
+    u = 0.5 + torch.rand(3, cols, device="cuda", generator=torch.Generator(device="cuda").manual_seed(9))
+    check_norm_f32(torch, k, u * torch.tensor([[1e-35], [1e-36], [1e-33]], device="cuda"), torch.full((cols,), 1e-4, device="cuda"), 1e-30)
+
+
 # ------------------------------------------------------------------------------------------ gemm
 def operand(torch, g, rows, cols, pad, offset=0):
     v, _ = rows_of(torch, rows, cols, pad, torch.int8, fill=77, offset=offset)
