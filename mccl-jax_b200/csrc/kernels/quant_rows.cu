@@ -476,22 +476,20 @@ __global__ void __launch_bounds__(kMaxThreads) quant_long_rows_kernel(const RowA
     if constexpr (NORM) return v * to_f32(w[j]);
     else return v;
   };
-  float ss = 0.f;
+  // a thread's squares in 64 bits: thousands of them added one by one in 32 would all be rounded the same way
+  double sum = 0.0;
   uint32_t mx = 0;
   for (long long j = threadIdx.x; j < a.cols; j += blockDim.x) {
     const float v = value(j, true);
-    ss = fmaf(v, v, ss);
+    if constexpr (NORM) sum = fma((double)v, (double)v, sum);
     mx = max(mx, abs_bits(t_of(v, j)));
   }
+  float ss = (float)sum;
   reduce_row<0, NORM, 0>(ss, mx);
   float down = 1.f;
   if constexpr (NORM) {
     if (abs_bits(ss) >= kInfBits && mx < kInfBits) {
-      ss = 0.f;
-      for (long long j = threadIdx.x; j < a.cols; j += blockDim.x) {
-        const float v = value(j, false) * kDown;
-        ss = fmaf(v, v, ss);
-      }
+      ss = (float)(sum * ((double)kDown * (double)kDown));
       uint32_t none = 0;
       reduce_row<0, true, 1>(ss, none);
       down = kDown;

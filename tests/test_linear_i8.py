@@ -297,6 +297,15 @@ def test_rms_norm_small_products(k, cuda, cols):
     check_norm_f32(torch, k, u * torch.tensor([[1e-35], [1e-36], [1e-33]], device="cuda"), torch.full((cols,), 1e-4, device="cuda"), 1e-30)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [200000, 3000001])
+def test_rms_norm_long_sums(k, cuda, cols):
+    """Equal values: the roundings of a sum in 32 bits would not cancel."""
+    torch = cuda
+    check_norm_f32(torch, k, torch.tensor([[1.1], [0.3], [1.7], [3e19]], device="cuda").expand(4, cols).contiguous(),
+                   torch.ones(cols, device="cuda"), 1e-5)
+
+
 # ------------------------------------------------------------------------------------------ gemm
 def operand(torch, g, rows, cols, pad, offset=0):
     v, _ = rows_of(torch, rows, cols, pad, torch.int8, fill=77, offset=offset)
