@@ -3493,18 +3493,19 @@ class Lowerer {
   }
 
   // Materialises `v` permuted by `perm` (and converted to out_dt) into a new slot.  With
-  // `inner_pitch` > 0 the innermost dim is stored with that row pitch (elements), leaving the pad
-  // columns unwritten: used to give TMA a 16-byte-aligned row stride.
+  // `inner_pitch` > 0 the rows that the last `inner_dims` dims make up (none: single elements) are
+  // stored with that pitch (elements), leaving the pad columns unwritten: used to give TMA a
+  // 16-byte-aligned row stride.
   int EmitPermute(const Value* v, const std::vector<int>& perm, const std::vector<int64_t>& out_dims, DT out_dt,
-                  int64_t inner_pitch = 0) {
+                  int64_t inner_pitch = 0, size_t inner_dims = 1) {
     int src = SlotFor(v);
-    int64_t n = 1;
+    int64_t n = 1, inner = 1;
     for (int64_t d : out_dims) n *= d;
-    const int64_t inner = out_dims.empty() ? 1 : out_dims.back();
+    for (size_t k = 0; k < std::min(inner_dims, out_dims.size()); ++k) inner *= out_dims[out_dims.size() - 1 - k];
     const int64_t pitch = inner_pitch > 0 ? inner_pitch : inner;
     int dst = NewSlot(n / std::max<int64_t>(inner, 1) * pitch * DTBytes(out_dt));
     const int rank = (int)perm.size();
-    if (rank >= 2 && perm.back() != rank - 1 && n > 0) {
+    if (rank >= 2 && perm.back() != rank - 1 && n > 0 && (inner_dims == 1 || pitch == inner)) {
       EmitTiledTranspose(v, perm, out_dims, out_dt, pitch, src, dst);
       return dst;
     }
@@ -3633,7 +3634,7 @@ class Lowerer {
       std::vector<int> perm(kord.begin(), kord.end());
       std::vector<int64_t> od;
       for (int q : perm) od.push_back(v->type.dims[q]);
-      return {EmitPermute(v, perm, od, ab, pitch), false, pitch ? pitch : g.K, ab};
+      return {EmitPermute(v, perm, od, ab, pitch, ct.size()), false, pitch ? pitch : g.K, ab};
     };
     Opnd oa = operand(a, lb, lf, lc, g.M), ob = operand(b, rb, rf, rc, g.N);
     g.a = oa.slot;
