@@ -3683,20 +3683,17 @@ class Lowerer {
     if (g.K > b200k::kGemmI8MaxK)
       throw LowerError{"dot_general on 8-bit integers sums at most " + std::to_string(b200k::kGemmI8MaxK) + " products"};
     const int64_t pitch = (g.K + 15) / 16 * 16;
-    auto operand = [&](const Value* v, std::vector<int64_t> order, const std::vector<int64_t>& fr,
+    auto operand = [&](const Value* v, const std::vector<int64_t>& bat, const std::vector<int64_t>& fr,
                        const std::vector<int64_t>& ct) -> std::pair<int, int64_t> {
-      order.insert(order.end(), fr.begin(), fr.end());
-      order.insert(order.end(), ct.begin(), ct.end());
+      std::vector<int> perm(bat.begin(), bat.end());
+      perm.insert(perm.end(), fr.begin(), fr.end());
+      perm.insert(perm.end(), ct.begin(), ct.end());
       bool in_order = true;
-      for (size_t k = 0; k < order.size(); ++k) in_order = in_order && order[k] == (int64_t)k;
+      for (size_t k = 0; k < perm.size(); ++k) in_order = in_order && perm[k] == (int)k;
       if (in_order && g.K == pitch) return {SlotFor(v), g.K};
-      // one row of K after the other, K as the innermost dimension also where it is several of v's or none
-      std::vector<int> perm(order.begin(), order.end());
       std::vector<int64_t> dims;
       for (int k : perm) dims.push_back(v->type.dims[k]);
-      if (ct.size() == 1 || g.K == pitch) return {EmitPermute(v, perm, dims, DT::kS8, ct.size() == 1 ? pitch : 0), ct.size() == 1 ? pitch : g.K};
-      throw LowerError{"dot_general on 8-bit integers: contracting " + std::to_string(ct.size()) +
-                       " dimensions of together " + std::to_string(g.K) + " elements (no multiple of 16)"};
+      return {EmitPermute(v, perm, dims, DT::kS8, pitch, ct.size()), pitch};
     };
     std::tie(g.a, g.lda) = operand(op->operands[0], lb, lf, lc);
     std::tie(g.b, g.ldb) = operand(op->operands[1], rb, rf, rc);

@@ -55,3 +55,43 @@ def test_products(client, name, dtype):
     ins = [rng.standard_normal(s).astype(ml_dtypes.bfloat16 if dtype == "bf16" else np.float16) for s in CASES[name][:2]]
     text = program(name, dtype, "f32")
     assert_close(client.run(text, ins)[0], oracle_run(text, ins)[0], RTOL_BF16)
+
+
+@pytest.mark.parametrize("name", sorted(CASES))
+def test_pitches_i8(lib_path, tmp_path, monkeypatch, name):
+    check_pitches(lib_path, tmp_path, monkeypatch, name, "i8", "i32", 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", sorted(CASES))
+def test_sums_i8(client, name):
+    rng = np.random.default_rng(8)
+    ins = [rng.integers(-128, 128, s, dtype=np.int8) for s in CASES[name][:2]]
+    text = program(name, "i8", "i32")
+    np.testing.assert_array_equal(client.run(text, ins)[0], oracle_run(text, ins)[0])
+
+
+def no_depth_program():
+    b = Builder("jit_no_depth")
+    x, w = b.arg((5, 0, 3), "i8"), b.arg((0, 7, 3), "i8")
+    return b.text([b.dot_general(x, w, contract=([1, 2], [0, 2]), out_dtype="i32")])
+
+
+def scalars_program():
+    b = Builder("jit_scalars")
+    x, w = b.arg((), "i8"), b.arg((), "i8")
+    return b.text([b.dot_general(x, w, contract=([], []), out_dtype="i32")])
+
+
+@pytest.mark.parametrize("text", [no_depth_program(), scalars_program()], ids=["no_depth", "scalars"])
+def test_smallest_plans_i8(lib_path, text):
+    rc, rep = report(lib_path, text)
+    assert rc == 0 and " i8" in rep, rep
+
+
+@pytest.mark.gpu
+def test_smallest_i8(client):
+    (got,) = client.run(no_depth_program(), [np.zeros((5, 0, 3), np.int8), np.zeros((0, 7, 3), np.int8)])
+    np.testing.assert_array_equal(got, np.zeros((5, 7), np.int32))
+    (got,) = client.run(scalars_program(), [np.int8(-128), np.int8(-7)])
+    assert int(got) == 896
