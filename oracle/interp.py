@@ -254,7 +254,7 @@ def dot_general(a, b, lb, rb, lc, rc, out_t):
     lf = [i for i in range(a.ndim) if i not in lb + lc]
     rf = [i for i in range(b.ndim) if i not in rb + rc]
     # integers are multiplied and added wide and wrap in the result's type, as if computed in it
-    wide = (lambda x: x.astype(np.int64)) if a.dtype.kind in "iu" else _hi
+    wide = (lambda x: x.astype(np.int64)) if a.dtype.kind in "iu" and b.dtype.kind in "iu" else _hi
     A = np.transpose(wide(a), lb + lf + lc)
     B = np.transpose(wide(b), rb + rc + rf)
     nb = int(np.prod([a.shape[i] for i in lb])) if lb else 1

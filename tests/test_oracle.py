@@ -175,3 +175,12 @@ def test_oracle_rejects_groups_that_miss_a_rank():
     ar = ('"stablehlo.all_reduce"(%arg0) <{replica_groups = dense<[[0, 1]]> : tensor<1x2xi64>}> ' + ADD_REGION)
     with pytest.raises(ValueError):
         run_spmd(_coll_prog(ar, "4", "4"), [[np.zeros(4, np.float32)] for _ in range(3)])
+
+
+@pytest.mark.parametrize("swap", [False, True])
+def test_dot_of_integers_and_floats(swap):
+    """An integer operand beside a float one: the products are floating."""
+    from oracle.interp import dot_general
+    a, b = np.array([[3, -2]], np.int8), np.array([[0.5], [0.25]], np.float32)
+    x, y = (b.T, a.T.copy()) if swap else (a, b)
+    np.testing.assert_array_equal(dot_general(x, y, [], [], [1], [0], "f32"), [[1.0]])
