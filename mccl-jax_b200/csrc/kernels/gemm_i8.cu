@@ -32,6 +32,7 @@
 namespace b200k {
 
 static __device__ int g_tc_error_gemm_i8;
+static std::atomic<bool> g_waits_launched{false};   // a kernel that may set the flag; for the rest of the process
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -765,6 +766,7 @@ int LaunchClusters(Kernel* kernel, int grid, int threads, int cluster, int smem,
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  g_waits_launched.store(true);
   return Launched(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
@@ -906,7 +908,9 @@ int OutCodeI8(int type) {
 
 }  // namespace
 
+// (Reading the flag blocks: executions without an 8-bit product, which ask too, are spared it.)
 int TakeGemmI8Error() {
+  if (!g_waits_launched.load()) return 0;
   int v = 0, z = 0;
   cudaMemcpyFromSymbol(&v, g_tc_error_gemm_i8, sizeof(int));
   if (v) cudaMemcpyToSymbol(g_tc_error_gemm_i8, &z, sizeof(int));

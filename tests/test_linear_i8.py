@@ -583,3 +583,39 @@ def test_offsets_past_32_bits(k, cuda):
     k.gemm_i8(q.data_ptr(), cols, b.data_ptr(), 48, scale.data_ptr(), None, None, c.data_ptr(), cols, rows, cols, 48, BF16, 0, None, 0,
               stream(torch))
     check_gemm(torch, c[at], *gemm_reference(torch, q[at][:, :48], b, scale[at], None, None, False), BF16, False)
+
+
+COUNT_READS = """
+import ctypes, sys
+import torch
+from torch.profiler import ProfilerActivity, profile
+sys.path.insert(0, sys.argv[2])
+from pjrt_b200 import kernels
+lib, k = ctypes.CDLL(sys.argv[1]), kernels.Kernels(sys.argv[1])
+a = torch.ones(300, 64, device="cuda", dtype=torch.int8)
+c = torch.empty(300, 300, device="cuda", dtype=torch.int32)
+def reads():
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        assert lib.b200_take_device_error() == 0
+        torch.cuda.synchronize()
+    return sum("Memcpy DtoH" in e.name for e in p.events())
+reads()
+before = reads()
+k.gemm_i8(a.data_ptr(), 64, a.data_ptr(), 64, None, None, None, c.data_ptr(), 300, 300, 300, 64, 4)
+print("reads", before, reads())
+"""
+
+
+@pytest.mark.gpu
+def test_error_flag_read_only_behind_products(lib_path, cuda):
+    """b200_take_device_error copies the 8-bit product's flag from the device once a product has been launched, and
+    before that the four flags of the other kernels alone."""
+    import subprocess
+    import sys
+    from conftest import PKG
+    r = subprocess.run([sys.executable, "-c", COUNT_READS, lib_path, PKG], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    before, after = (int(n) for n in r.stdout.split("reads")[1].split())
+    if not after:
+        pytest.skip("copies are not recorded here")
+    assert (before, after) == (4, 5)
