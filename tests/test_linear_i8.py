@@ -619,3 +619,105 @@ def test_error_flag_read_only_behind_products(lib_path, cuda):
     if not after:
         pytest.skip("copies are not recorded here")
     assert (before, after) == (4, 5)
+
+
+# ------------------------------------------------------------------------------------------ every launch form
+def row_pitch(cols, aligned):
+    """Rows 16-byte aligned, or at odd places."""
+    return (cols + 15) // 8 * 8 if aligned else cols + 1 + cols % 2
+
+
+# with 1200 rows and with three: rows in 1 to 4 groups of eight a lane, in blocks of up to 256, 512 and 1024 threads
+WIDTHS = [301, 701, 1003, 1501, 2041, 3501, 5003, 12005, 20011]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [3, 1200])
+@pytest.mark.parametrize("cols", WIDTHS)
+@pytest.mark.parametrize("aligned", [True, False])
+def test_quantize_every_form(k, cuda, dtype, rows, cols, aligned):
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(rows * 139 + cols)
+    ld = row_pitch(cols, aligned)
+    x = activations(torch, g, rows, cols, ld - cols, types(torch)[dtype])
+    q, flat = rows_of(torch, rows, cols, ld - cols, torch.int8, fill=99)
+    scale = torch.empty(rows, device="cuda")
+    k.quantize_i8(x.data_ptr(), ld, q.data_ptr(), ld, scale.data_ptr(), rows, cols, dtype, stream(torch))
+    ref, m = rounded(torch, x.float())
+    assert torch.equal(q, ref)
+    close_f32(torch, scale, m.double() / 127.0, 1)
+    flat[:rows * ld].view(rows, ld)[:, :cols] = 99
+    assert bool((flat == 99).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,wtype", [(BF16, BF16), (F16, F32), (F32, F32)])
+@pytest.mark.parametrize("rows", [3, 1200])
+@pytest.mark.parametrize("cols", WIDTHS)
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("form", ["written", "over_x"])
+def test_rms_norm_every_form(k, cuda, dtype, wtype, rows, cols, aligned, form):
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(rows * 149 + cols)
+    t, ld = types(torch), row_pitch(cols, aligned)
+    x, r = (activations(torch, g, rows, cols, ld - cols, t[dtype]) for _ in range(2))
+    w = (1.0 + 0.3 * torch.randn(cols, device="cuda", generator=g)).to(t[wtype])
+    ref_h, ref_q, ref_scale = norm_reference(torch, x, r, w, 1e-5)
+    h = x if form == "over_x" else rows_of(torch, rows, cols, ld - cols, t[dtype])[0]
+    q, flat = rows_of(torch, rows, cols, ld - cols, torch.int8, fill=99)
+    scale = torch.empty(rows, device="cuda")
+    k.rms_norm_i8(x.data_ptr(), ld, r.data_ptr(), ld, w.data_ptr(), h.data_ptr(), ld, q.data_ptr(), ld, scale.data_ptr(), rows, cols,
+                  dtype, wtype, 1e-5, stream(torch))
+    assert torch.equal(h, ref_h) and torch.equal(q, ref_q)
+    close_f32(torch, scale, ref_scale, (math.log2(cols) + 34) / 2 + 4)
+    flat[:rows * ld].view(rows, ld)[:, :cols] = 99
+    assert bool((flat == 99).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [16, 1001, 6000, 40000])
+def test_rms_norm_large_values_and_weights(k, cuda, cols):
+    """Squares that overflow beside weights as large: the scale is finite, and no step on the way to it overflows."""
+    torch = cuda
+    u = 0.5 + 0.5 * torch.rand(1, cols, device="cuda", generator=torch.Generator(device="cuda").manual_seed(7))
+    check_norm_f32(torch, k, 1e20 * u, torch.full((cols,), 1e18, device="cuda"), 1e-5)
+
+
+def check_every_result(torch, k, m, n, kk, pad, npad):
+    """The product in every type, with and without GELU and in raw sums: all of C, and what lies between its rows."""
+    g = torch.Generator(device="cuda").manual_seed(m * 41 + n * 13 + kk)
+    a, b = operand(torch, g, m, kk, pad), operand(torch, g, n, kk, pad)
+    s, size = scratch_for(torch, k, a, kk + pad, b, kk + pad, m, n, kk)
+    sa = (0.5 + torch.rand(m, device="cuda", generator=g)) * 0.05
+    sb = (0.5 + torch.rand(n, device="cuda", generator=g)) * 20 / (5000.0 * math.sqrt(kk))
+    bias = torch.randn(n, device="cuda", generator=g)
+    for out_type, act in ((S32, 0), (F32, 0), (F32, 1), (BF16, 0), (BF16, 1), (F16, 0), (F16, 1)):
+        c, flat = rows_of(torch, m, n, npad, torch.int32 if out_type == S32 else types(torch)[out_type], fill=99)
+        ptrs = [None] * 3 if out_type == S32 else [t.data_ptr() for t in (sa, sb, bias)]
+        k.gemm_i8(a.data_ptr(), kk + pad, b.data_ptr(), kk + pad, *ptrs, c.data_ptr(), n + npad, m, n, kk, out_type, act, s.data_ptr(),
+                  size, stream(torch))
+        if out_type == S32:
+            assert torch.equal(c.double(), a.double() @ b.double().t())
+        else:
+            check_gemm(torch, c, *gemm_reference(torch, a, b, sa, sb, bias, bool(act)), out_type, bool(act))
+        flat[:m * (n + npad)].view(m, n + npad)[:, :n] = 99
+        assert bool((flat == 99).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,kk,pad", [(4500, 4096, 1000, 8), (4500, 4100, 1000, 0), (8192, 2301, 768, 0), (5000, 4104, 130, 14)])
+@pytest.mark.parametrize("npad", [0, 8, 3])
+def test_gemm_many_tiles_a_pair(k, cuda, monkeypatch, m, n, kk, pad, npad):
+    """Pairs of CTAs that work on three and more tiles each, with K in more blocks than a tile has stages and in fewer,
+    rows of C that TMA can write and that it cannot."""
+    monkeypatch.setenv("B200_GEMM_I8_FORM", "pair")
+    check_every_result(cuda, k, m, n, kk, pad, npad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["pair", "0x1", "0x4", "32x1", "32x6", "64x1", "64x2", "128x1", "128x3"])
+@pytest.mark.parametrize("m,n,kk", [(1, 300, 1500), (7, 515, 768), (70, 130, 1024), (300, 520, 1000)])
+def test_gemm_every_form_and_result(k, cuda, monkeypatch, form, m, n, kk):
+    monkeypatch.setenv("B200_GEMM_I8_FORM", form)
+    check_every_result(cuda, k, m, n, kk, 0, 3)
