@@ -339,7 +339,7 @@ __device__ __forceinline__ float row_scale(uint32_t mx, float ss, float down, in
 // holds the group before them once more: the lines that two groups share are then written by one lane wherever
 // they lie, and only a row's two ends are written element by element.
 template <typename T, typename W, bool NORM, bool ALIGNED, int NG, int LANES, int MAXT>
-__global__ void __launch_bounds__(MAXT, NORM && NG == 4 && MAXT == 256 && sizeof(T) + sizeof(W) == 4 ? 3 : 0) quant_rows_kernel(const RowArgs a) {
+__global__ void __launch_bounds__(MAXT, NORM && NG == 4 && MAXT == 256 ? 3 : 0) quant_rows_kernel(const RowArgs a) {
   constexpr int kLanes = LANES ? LANES : 32;
   const int tid = LANES ? (int)(threadIdx.x & (kLanes - 1)) : (int)threadIdx.x;
   const int step = LANES ? kLanes : (int)blockDim.x;
@@ -502,13 +502,18 @@ __global__ void __launch_bounds__(kMaxThreads) quant_long_rows_kernel(const RowA
     q[j] = (int8_t)(s.live ? round_i8(t_of(value(j, false), j), s.inv, s.m) : 0u);
 }
 
-template <typename T, typename W, bool NORM, bool ALIGNED, int NG>
+// FROM and TO: the smallest and the largest block that the caller's rows come to.
+template <typename T, typename W, bool NORM, bool ALIGNED, int NG, int FROM = 256, int TO = kMaxThreads>
 void LaunchBlock(const RowArgs& a, int groups, cudaStream_t st) {
   // not aligned: 31 groups a warp, and a lane past the last group, which writes the end of its last line
   const int per = ALIGNED ? 32 * NG : 31 * NG, threads = ((groups + (ALIGNED ? 0 : 1) + per - 1) / per) * 32;
-  if (threads <= 256) quant_rows_kernel<T, W, NORM, ALIGNED, NG, 0, 256><<<a.rows, threads, 0, st>>>(a);
-  else if (threads <= 512) quant_rows_kernel<T, W, NORM, ALIGNED, NG, 0, 512><<<a.rows, threads, 0, st>>>(a);
-  else quant_rows_kernel<T, W, NORM, ALIGNED, NG, 0, kMaxThreads><<<a.rows, threads, 0, st>>>(a);
+  if constexpr (FROM <= 256) {
+    if (TO == 256 || threads <= 256) return quant_rows_kernel<T, W, NORM, ALIGNED, NG, 0, 256><<<a.rows, threads, 0, st>>>(a);
+  }
+  if constexpr (FROM <= 512 && TO >= 512) {
+    if (TO == 512 || threads <= 512) return quant_rows_kernel<T, W, NORM, ALIGNED, NG, 0, 512><<<a.rows, threads, 0, st>>>(a);
+  }
+  if constexpr (TO > 512) quant_rows_kernel<T, W, NORM, ALIGNED, NG, 0, kMaxThreads><<<a.rows, threads, 0, st>>>(a);
 }
 template <typename T, typename W, bool NORM, bool ALIGNED, int NG, int LANES>
 void LaunchWarp(const RowArgs& a, cudaStream_t st) {
@@ -531,17 +536,25 @@ void LaunchTW(const RowArgs& a, cudaStream_t st) {
     if (!many && groups <= kMaxThreads) return LaunchBlock<T, W, NORM, true, 1>(a, groups, st);
     if (groups <= 64) return LaunchWarp<T, W, NORM, true, 2, 32>(a, st);
     if (groups <= 96) return LaunchWarp<T, W, NORM, true, 3, 32>(a, st);
-    if (!NORM && groups <= 128) return LaunchWarp<T, W, NORM, true, 4, 32>(a, st);
-    // (more than 512 groups of 16-bit values: four, in blocks of at most 256 threads, three to an SM; 8192 x 8192
-    // bf16: 84 us, with two groups and 512 threads 93)
-    if (NORM && sizeof(T) + sizeof(W) == 4 && groups > 512 && groups <= 1024) return LaunchBlock<T, W, NORM, true, 4>(a, groups, st);
-    if (NORM && groups <= 2 * kMaxThreads) return LaunchBlock<T, W, NORM, true, 2>(a, groups, st);
-    if (groups <= 4 * kMaxThreads) return LaunchBlock<T, W, NORM, true, 4>(a, groups, st);
+    if constexpr (NORM && sizeof(T) + sizeof(W) == 4) {
+      // (more than 512 groups of 16-bit values: four, in blocks of at most 256 threads, three to an SM; 8192 x 8192
+      // bf16: 84 us, with two groups and 512 threads 93)
+      if (groups <= 512) return LaunchBlock<T, W, true, true, 2, 256, 256>(a, groups, st);
+      if (groups <= 1024) return LaunchBlock<T, W, true, true, 4, 256, 256>(a, groups, st);
+      if (groups <= 2 * kMaxThreads) return LaunchBlock<T, W, true, true, 2, kMaxThreads>(a, groups, st);
+      if (groups <= 4 * kMaxThreads) return LaunchBlock<T, W, true, true, 4, kMaxThreads>(a, groups, st);
+    } else if constexpr (NORM) {
+      if (groups <= 2 * kMaxThreads) return LaunchBlock<T, W, true, true, 2>(a, groups, st);
+      if (groups <= 4 * kMaxThreads) return LaunchBlock<T, W, true, true, 4, kMaxThreads>(a, groups, st);
+    } else {
+      if (groups <= 128) return LaunchWarp<T, W, false, true, 4, 32>(a, st);
+      if (groups <= 4 * kMaxThreads) return LaunchBlock<T, W, false, true, 4>(a, groups, st);
+    }
   } else {
     // bf16 16384 x 4096 norm: 172 and 140 us with 1 and 2 groups; 8192 x 1003: 25 and 29 us
     if (groups <= 256 || (!(NORM && many) && lanes <= kMaxThreads / 32 * 31)) return LaunchBlock<T, W, NORM, false, 1>(a, groups, st);
-    if (lanes <= kMaxThreads / 32 * 31 * 2) return LaunchBlock<T, W, NORM, false, 2>(a, groups, st);
-    if (lanes <= kMaxThreads / 32 * 31 * 4) return LaunchBlock<T, W, NORM, false, 4>(a, groups, st);
+    if (lanes <= kMaxThreads / 32 * 31 * 2) return LaunchBlock<T, W, NORM, false, 2, NORM ? 256 : kMaxThreads>(a, groups, st);
+    if (lanes <= kMaxThreads / 32 * 31 * 4) return LaunchBlock<T, W, NORM, false, 4, kMaxThreads>(a, groups, st);
   }
   quant_long_rows_kernel<T, W, NORM><<<a.rows, kMaxThreads, 0, st>>>(a);
 }
