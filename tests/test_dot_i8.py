@@ -93,3 +93,21 @@ def test_scaled_linear_layer(client):
     ins = [rng.integers(-128, 128, (m, k), dtype=np.int8), rng.integers(-128, 128, (n, k), dtype=np.int8),
            rng.random(m).astype(np.float32), rng.random(n).astype(np.float32)]
     assert_close(client.run(text, ins)[0], oracle_run(text, ins)[0], RTOL_F32)
+
+
+def computed_program(m, n, k):
+    """Operands that the program computes: x rounded to 8 bits, w transposed."""
+    b = Builder("jit_computed_i8")
+    x, w = b.arg((m, k), "f32"), b.arg((k, n), "i8")
+    q = b.convert(x * 2.0, "i8")
+    return b.text([b.dot_general(q, b.transpose(w, [1, 0]), contract=([1], [1]), out_dtype="i32"), q])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(37, 53, 75), (1, 40, 33), (130, 64, 64)])
+def test_computed_operands(client, m, n, k):
+    rng = np.random.default_rng(6)
+    ins = [rng.integers(-60, 61, (m, k)).astype(np.float32), rng.integers(-128, 128, (k, n), dtype=np.int8)]
+    text = computed_program(m, n, k)
+    for got, ref in zip(client.run(text, ins), oracle_run(text, ins)):
+        np.testing.assert_array_equal(got, ref)

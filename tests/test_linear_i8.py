@@ -721,3 +721,27 @@ def test_gemm_many_tiles_a_pair(k, cuda, monkeypatch, m, n, kk, pad, npad):
 def test_gemm_every_form_and_result(k, cuda, monkeypatch, form, m, n, kk):
     monkeypatch.setenv("B200_GEMM_I8_FORM", form)
     check_every_result(cuda, k, m, n, kk, 0, 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["pair", "0x8", "32x1", "32x8", "64x4", "128x1"])
+@pytest.mark.parametrize("m", [4, 100])
+def test_gemm_deepest_sum_in_every_form(k, cuda, monkeypatch, form, m):
+    torch = cuda
+    monkeypatch.setenv("B200_GEMM_I8_FORM", form)
+    kk, n = 131071, 130
+    a = torch.full((m, kk), -128, device="cuda", dtype=torch.int8)
+    b = torch.full((n, kk), -128, device="cuda", dtype=torch.int8)
+    b[1::2] = 127
+    c = torch.empty(m, n, device="cuda", dtype=torch.int32)
+    s, size = scratch_for(torch, k, a, kk, b, kk, m, n, kk)
+    k.gemm_i8(a.data_ptr(), kk, b.data_ptr(), kk, None, None, None, c.data_ptr(), n, m, n, kk, S32, 0, s.data_ptr(), size, stream(torch))
+    assert bool((c[:, ::2] == 16384 * kk).all()) and bool((c[:, 1::2] == -128 * 127 * kk).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["pair", "0x1", "32x1", "64x1", "128x1"])
+@pytest.mark.parametrize("m,n,kk", [(1, 1, 1), (5, 1, 1), (100, 1, 17), (3, 7, 1), (300, 1, 256)])
+def test_gemm_smallest_in_every_form(k, cuda, monkeypatch, form, m, n, kk):
+    monkeypatch.setenv("B200_GEMM_I8_FORM", form)
+    check_every_result(cuda, k, m, n, kk, 0, 0)
