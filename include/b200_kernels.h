@@ -62,7 +62,8 @@ B200_API int b200_gemm_split(const void* A, int a_type, const void* B, int b_typ
 
 /* q[i][j] = round_half_even(127 x[i][j] / max_j |x[i][j]|), the exact quotient's rounding, and scale[i] =
  * max_j |x[i][j]| / 127, so x is about q * scale.  dtype (of x) in {F32, BF16, F16}.  A row of zeros gives
- * scale 0 and q 0, a row holding an infinity or a NaN scale NaN and q 0.  rows or cols may be 0. */
+ * scale 0 and q 0, a row holding an infinity or a NaN scale NaN and q 0.  rows or cols may be 0, and are below
+ * 2^31. */
 B200_API int b200_quantize_i8(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows,
                               int64_t cols, int dtype, void* stream);
 
@@ -71,14 +72,16 @@ B200_API int b200_quantize_i8(const void* x, int64_t ldx, int8_t* q, int64_t ldq
  * max_j |t| / 127 / sqrt(mean_j h^2 + eps), so the normalised row is about q * scale.  weight [cols] of
  * weight_dtype; x, residual and h of dtype, each in {F32, BF16, F16}.  residual may be NULL, and then h is
  * NULL too; with a residual h may be NULL (not written), or x or residual themselves with their pitch (no other overlap).
- * eps > 0.  A row whose t holds an infinity or a NaN gives scale NaN and q 0.  rows may be 0. */
+ * eps > 0 (squares are f32: below 2^-126 it no longer covers what they lose).  A row whose t holds an infinity or a
+ * NaN gives scale NaN and q 0.  rows may be 0; rows and cols are below 2^31. */
 B200_API int b200_rms_norm_i8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* h,
                               int64_t ldh, int8_t* q, int64_t ldq, float* scale, int64_t rows, int64_t cols, int dtype,
                               int weight_dtype, float eps, void* stream);
 
 /* C[i][j] = act(f32(sum_k A[i][k] B[j][k]) a_scale[i] b_scale[j] + bias[j]): A [M, K] and B [N, K] of 8-bit
  * integers, K contiguous, the sum exact in 32 bits (K <= 131071), C [M, N] of out_type in {F32, BF16, F16},
- * act B200_ACT_NONE or B200_ACT_GELU (its tanh form).  a_scale [M], b_scale [N] and bias [N] are f32 and may
+ * act B200_ACT_NONE or B200_ACT_GELU (its tanh form).  The products are f32, from the left: the sum times a_scale[i]
+ * has to be finite.  M and N are at most 2^31 - 257.  a_scale [M], b_scale [N] and bias [N] are f32 and may
  * each be NULL (1, 1, 0).  out_type S32 gives the sums themselves, without scales, bias or act.  Any of M, N,
  * K may be 0.  An operand whose address or pitch is no multiple of 16 bytes is first copied to such rows in
  * `scratch`, 256-byte aligned device memory of b200_gemm_i8_scratch_bytes(...) bytes for these operands (0, and

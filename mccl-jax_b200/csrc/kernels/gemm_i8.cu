@@ -849,7 +849,9 @@ int LaunchForm(const Call& c, const Form& f) {
 // `fixed` plus `block` for each 128 of K, and half of that again for each further CTA its SM holds (two at a time
 // share its loads); adding 2^i slices of K costs 0.76 i; pairs take 7.5 plus 0.333 for each round and 128 of K.
 // Fitted to the times of 13 forms at 37 sizes from 4 x 1000 x 1000 to 8192 x 768 x 768 and 1024 x 8192 x 8192: the
-// form it picks takes 4 % longer than the best of the 13 on average.
+// form it picks takes 4 % longer than the best of the 13 on average, 17 % at most (8192 x 64 x 4096).  Pairs were timed
+// from 64 tokens on; below, the model's word for them is taken unfitted (8 x 50257 x 768: 17.7 us where tiles of 32
+// tokens take 14.9).
 Form ChooseForm(int64_t M, int64_t N, int64_t K, int sms) {
   Form f;
   const int64_t kbs = (K + BK - 1) / BK;

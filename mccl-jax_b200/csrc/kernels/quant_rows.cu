@@ -15,7 +15,7 @@
 // like the values with infinity and NaN on top: a row that holds either is seen by the same reduction.
 //
 // HBM bounds it: read and written once are 7 bytes an element for a bf16 norm with residual, 3 for bf16 rows.
-// Measured on B200: norm [8192, 8192] bf16 84 us (5.6 TB/s), [8192, 8192] f32 133 us (6.6 TB/s), quantize
+// Measured on B200: norm [8192, 8192] bf16 84-87 us (5.4-5.6 TB/s), [8192, 8192] f32 133 us (6.6 TB/s), quantize
 // [50257, 768] f32 31 us (6.2 TB/s), [16384, 4096] bf16 41 us (4.9 TB/s); one row of 768: 2 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
