@@ -3682,6 +3682,8 @@ class Lowerer {
                  const std::vector<int64_t>& rc) {
     if (g.K > b200k::kGemmI8MaxK)
       throw LowerError{"dot_general on 8-bit integers sums at most " + std::to_string(b200k::kGemmI8MaxK) + " products"};
+    if (g.M > b200k::kGemmI8MaxRows || g.N > b200k::kGemmI8MaxRows)
+      throw LowerError{"dot_general on 8-bit integers takes at most " + std::to_string(b200k::kGemmI8MaxRows) + " rows"};
     const int64_t pitch = (g.K + 15) / 16 * 16;
     auto operand = [&](const Value* v, const std::vector<int64_t>& bat, const std::vector<int64_t>& fr,
                        const std::vector<int64_t>& ct) -> std::pair<int, int64_t> {

@@ -928,7 +928,7 @@ int GemmI8(const void* A, int64_t lda, const void* B, int64_t ldb, const float* 
            void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, int out_type, int act, void* scratch, size_t scratch_bytes,
            cudaStream_t st) {
   const int out = OutCodeI8(out_type);
-  if (out < 0 || M < 0 || N < 0 || K < 0 || M > INT32_MAX - 256 || N > INT32_MAX - 256 || K > kGemmI8MaxK || lda < K || ldb < K ||
+  if (out < 0 || M < 0 || N < 0 || K < 0 || M > kGemmI8MaxRows || N > kGemmI8MaxRows || K > kGemmI8MaxK || lda < K || ldb < K ||
       ldc < N)
     return -1;
   if (act < B200_ACT_NONE || act > B200_ACT_GELU || (out == kOutS32 && (a_scale || b_scale || bias || act))) return -1;

@@ -52,6 +52,7 @@ int GemmSplit(const void* A, long long lda, bool a_mn, int a_type, const void* B
 // The internal forms of b200_quantize_i8, b200_rms_norm_i8 and b200_gemm_i8 (include/b200_kernels.h).
 // 128 * 128 * kGemmI8MaxK is the largest sum a 32-bit integer holds.
 constexpr int64_t kGemmI8MaxK = 131071;
+constexpr int64_t kGemmI8MaxRows = 2147483391;    // of M and of N: a tile's last row is a 32-bit integer too
 int QuantizeI8(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int64_t rows, int64_t cols, int dtype,
                cudaStream_t st);
 int RmsNormI8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, void* h, int64_t ldh,

@@ -111,3 +111,18 @@ def test_computed_operands(client, m, n, k):
     text = computed_program(m, n, k)
     for got, ref in zip(client.run(text, ins), oracle_run(text, ins)):
         np.testing.assert_array_equal(got, ref)
+
+
+@pytest.mark.parametrize("m,n", [(2147483392, 1), (1, 2147483392)])
+def test_more_rows_than_a_launch_takes_are_refused(lib_path, m, n):
+    b = Builder("jit_tall")
+    x, w = b.arg((m, 16), "i8"), b.arg((n, 16), "i8")
+    rc, rep = report(lib_path, b.text([b.dot_general(x, w, contract=([1], [1]), out_dtype="i32")]))
+    assert rc != 0 and "at most 2147483391 rows" in rep, rep
+
+
+def test_most_rows(lib_path):
+    b = Builder("jit_tall")
+    x, w = b.arg((2147483391, 16), "i8"), b.arg((1, 16), "i8")
+    rc, rep = report(lib_path, b.text([b.dot_general(x, w, contract=([1], [1]), out_dtype="i32")]))
+    assert rc == 0, rep
